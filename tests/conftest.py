@@ -147,6 +147,8 @@ def pytest_terminal_summary(terminalreporter, exitstatus, config):
     HSA_STATUS_ERROR_ILLEGAL_INSTRUCTION queue abort; every such event is reported here so that it is visible in the
     tail of the test log (and in gpurun_out/one_device_retries.log on the GPU box)."""
     from tests import spawn_one_device
+    if not spawn_one_device.RETRIES:
+        return          # (a run without one does not print the runtime's message: who reads the log for it would find it)
     terminalreporter.write_line(f"one-device harness: {len(spawn_one_device.RETRIES)} rank re-run(s) on "
                                 f"{spawn_one_device.FAULT_TEXT}")
     for when, nprocs, line in spawn_one_device.RETRIES:
