@@ -16,7 +16,9 @@ _LAZY = {
     "BBBOptimizer": ".bbb", "GaussianPrior": ".bbb", "MixturePrior": ".bbb",
     "GaussianParameter": ".util", "normal_like": ".util", "reset_model_params": ".util",
     "iVONOptimizer": ".ivon",
-    "BBBLinear": ".bbb_layers", "BBBConv2d": ".bbb_layers", "make_module_bbb": ".bbb_layers",
+    "BBBLinear": ".bbb_layers", "BBBConv2d": ".bbb_layers", "BBBEmbedding": ".bbb_layers", "make_module_bbb": ".bbb_layers",
+    "embedding": ".lookup", "gaussian_embedding": ".lookup", "ScaledEmbedding": ".lookup",
+    "topk_logits": ".distill", "distillation_loss": ".distill", "TopLogits": ".distill",
     "DeepEnsemble": ".ensemble",
     "HipOps": ".ops",
 }

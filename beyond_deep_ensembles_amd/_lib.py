@@ -102,10 +102,22 @@ SIGNATURES = {
                                    c_int, c_int, c_int, _P, _P]),
     "bde_ivon_sample": (c_int, [_P, _P, _P, c_uint64, c_uint64, c_float, c_int, c_int, _P, _P, c_int64, _P]),
     "bde_ivon_update": (c_int, [_P, _P, _P, _P, _P] + [c_float] * 11 + [c_int64, _P]),
+    "bde_embedding_fwd": (c_int, [_P, c_int, c_int64, _P, c_int64, _P, c_int, _P, c_int64, c_int, c_uint64, c_uint64, c_float,
+                                  c_int64, _P, c_int, c_int64, c_int64, c_int64, _P]),
+    "bde_embedding_bwd_ws_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "bde_embedding_bwd": (c_int, [_P, c_int, c_int64, _P, c_int, _P, c_int64, _P, c_int64, c_int, c_uint64, c_uint64, c_float,
+                                  c_int64, _P, c_int, _P, c_int64, c_int64, c_int64, _P, c_size_t, _P]),
+    "bde_topk_limits": (c_int, [_P, _P]),
+    "bde_topk_logits": (c_int, [_P, c_int, c_int64, c_float, c_int, c_int, c_int, _P, _P, _P, _P]),
+    "bde_distill_limits": (c_int, [_P, _P]),
+    "bde_distill_fwd": (c_int, [_P, c_int, c_int64, _P, c_int, _P, c_int, _P, _P, c_int, c_float, c_float, c_int, c_int, c_int,
+                                _P, _P, _P, _P, _P]),
+    "bde_distill_bwd": (c_int, [_P, c_int, c_int64, _P, c_int, _P, c_int, _P, _P, _P, c_int, c_float, c_float, _P, c_int64, c_int,
+                                c_int, c_int, c_int, _P, _P]),
 }
 
 _lib = None
-ABI_VERSION = 406        # csrc/version.hip, include/bde_hip.h
+ABI_VERSION = 407        # csrc/version.hip, include/bde_hip.h
 
 
 class BdeLibraryError(RuntimeError):

@@ -34,6 +34,7 @@ from torch.autograd.function import once_differentiable
 import torch.nn.functional as F
 
 from . import _host
+from .lookup import gaussian_embedding
 from .util import GaussianParameter, normal_like, _philox_stream
 
 _CLAMP = 1e-4
@@ -521,10 +522,49 @@ class BBBConv2d(_LocalReparamLayer):
         return self._sample_activations(mean, var)
 
 
-def make_module_bbb(module: nn.Module, prior, **kwargs) -> int:
+class BBBEmbedding(_LocalReparamLayer):
+    """The mean-field embedding: a Gaussian table ``weight`` [num_embeddings, embedding_dim] looked up by token
+    (``gaussian_embedding``; no reference counterpart).  ``sampling="activations"``: every position has its own noise, as the
+    other layers' pre-activations do -- the layer is a linear one whose input is one-hot, so its output variance is the row's
+    own sigma^2 (not clamped).  In eval mode with ``freeze_on_eval`` all positions of a token share one draw per call, which
+    is ONE set of weights, and so does ``sampling="parameters"`` in either mode.  ``rng="philox"`` generates the noise in the
+    kernel, for the touched rows only.  Positions holding ``padding_idx`` have no noise and no gradient."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, weight_prior, padding_idx=None, *, scale=1.0, out_dtype=None, **kwargs):
+        super().__init__()
+        self.num_embeddings, self.embedding_dim = num_embeddings, embedding_dim
+        if padding_idx is not None and padding_idx < 0:
+            padding_idx += num_embeddings
+        if padding_idx is not None and not 0 <= padding_idx < num_embeddings:
+            raise ValueError(f"padding_idx outside the table of {num_embeddings} rows")
+        self.padding_idx, self.scale, self.out_dtype = padding_idx, float(scale), out_dtype
+        self._init_common((num_embeddings, embedding_dim), None, weight_prior, None, dict(kwargs, bias=False))
+
+    def reset_parameters(self):
+        super().reset_parameters()
+        if self.padding_idx is not None:
+            with torch.no_grad():
+                self.weight.mean[self.padding_idx].zero_()
+
+    def forward(self, tokens: torch.Tensor):
+        if self.sampling not in ("activations", "parameters"):
+            raise ValueError("Invalid value of sampling")
+        w = self.weight
+        shared = self.sampling == "parameters" or (not self.training and self.freeze_on_eval)
+        eps = None
+        if w.noise_source is not None and shared:
+            eps = w.noise_source(w.rho)
+        elif w.rng != "philox" or w.noise_source is not None:
+            eps = normal_like(w.rho.detach() if shared else w.rho.new_empty(tuple(tokens.shape) + (self.embedding_dim,)))
+        return gaussian_embedding(tokens, w.mean, w.rho, noise="token" if shared else "position", eps=eps, seed=w.seed, scale=self.scale,
+                                  padding_idx=self.padding_idx, out_dtype=self.out_dtype, _ops=w._get_ops())
+
+
+def make_module_bbb(module: nn.Module, prior, *, embeddings: bool = False, **kwargs) -> int:
     """Replace every nn.Linear / nn.Conv2d of ``module`` by its mean-field counterpart, keeping the
     current weights as the means (cf. the reference's ``make_module_bbb``); returns the number of
-    layers replaced."""
+    layers replaced.  ``embeddings=True`` replaces its nn.Embedding tables (plain lookups: no ``max_norm``,
+    ``scale_grad_by_freq``, ``sparse``; a ScaledEmbedding keeps its scale) by BBBEmbedding as well."""
     replaced = 0
     for name, child in list(module.named_children()):
         new = None
@@ -534,14 +574,18 @@ def make_module_bbb(module: nn.Module, prior, **kwargs) -> int:
                 and child.kernel_size[0] == child.kernel_size[1] and isinstance(child.padding, tuple):
             new = BBBConv2d(child.in_channels, child.out_channels, child.kernel_size[0], prior, prior,
                             stride=child.stride, padding=child.padding, bias=child.bias is not None, **kwargs)
+        elif embeddings and isinstance(child, nn.Embedding) and child.max_norm is None and not child.scale_grad_by_freq \
+                and not child.sparse and child.weight.dtype == torch.float32:
+            new = BBBEmbedding(child.num_embeddings, child.embedding_dim, prior, child.padding_idx, scale=getattr(child, "scale", 1.0),
+                               out_dtype=getattr(child, "out_dtype", None), **kwargs)
         if new is not None:
             new = new.to(child.weight.device)
             with torch.no_grad():
                 new.weight.mean.copy_(child.weight)
-                if child.bias is not None:
+                if getattr(child, "bias", None) is not None:
                     new.bias.mean.copy_(child.bias)
             setattr(module, name, new)
             replaced += 1
         else:
-            replaced += make_module_bbb(child, prior, **kwargs)
+            replaced += make_module_bbb(child, prior, embeddings=embeddings, **kwargs)
     return replaced

@@ -1,10 +1,12 @@
 #include "bde_common.hpp"
-extern "C" int bde_version(void) { return 406; /* 0.4.5: bde_svgd_step streams at every size (the small-model kernel is the caller's explicit choice), bde_mean_scalars multiplies by fl(1/divisor) like torch's GPU division, bde_conv_lrt_bwd_weight takes ws_bytes (0.4.4: + bde_conv_lrt_gvar_bias (g_var and the bias gradients in one pass) (0.4.3: + conv tuning hooks (bde_conv_lrt_pass_geos / _candidates / _set_tiling, _wgrad_candidates / _wgrad_set_tiling) (0.4.2: + bde_sum_scalars; conv weight gradient: one instantiation per column-tile count, 512-slot shares, tree reduction (0.4.1: + bde_conv_lrt_prep_strided / bde_conv_lrt_bwd_data_phases (0.4.0: contiguous SWAG rows again, LDS-DMA batched sampler, bde_conv_lrt_*, single-launch protocol gone))))) */ }
+extern "C" int bde_version(void) { return 407; /* 0.4.7: + bde_embedding_*, bde_topk_*, bde_distill_* (0.4.5: bde_svgd_step streams at every size (the small-model kernel is the caller's explicit choice), bde_mean_scalars multiplies by fl(1/divisor) like torch's GPU division, bde_conv_lrt_bwd_weight takes ws_bytes (0.4.4: + bde_conv_lrt_gvar_bias (g_var and the bias gradients in one pass) (0.4.3: + conv tuning hooks (bde_conv_lrt_pass_geos / _candidates / _set_tiling, _wgrad_candidates / _wgrad_set_tiling) (0.4.2: + bde_sum_scalars; conv weight gradient: one instantiation per column-tile count, 512-slot shares, tree reduction (0.4.1: + bde_conv_lrt_prep_strided / bde_conv_lrt_bwd_data_phases (0.4.0: contiguous SWAG rows again, LDS-DMA batched sampler, bde_conv_lrt_*, single-launch protocol gone)))))) */ }
 extern "C" const char* bde_arch(void) { return "gfx950"; }
 
 extern "C" {
 int bde_internal_load_conv_lrt(void);
 int bde_internal_load_conv_lrt_bwd(void);
+int bde_internal_load_distill(void);
+int bde_internal_load_embedding(void);
 int bde_internal_load_gauss(void);
 int bde_internal_load_ivon(void);
 int bde_internal_load_lrt(void);
@@ -14,6 +16,7 @@ int bde_internal_load_svgd_fused(void);
 int bde_internal_load_svgd_small(void);
 int bde_internal_load_swag(void);
 int bde_internal_load_swag_batched(void);
+int bde_internal_load_topk(void);
 }
 
 // Load every code object of the library on the CURRENT device.  HIP defers the upload of a code object to the first
@@ -31,7 +34,8 @@ static std::atomic<unsigned> g_optional_failures{0};
 
 extern "C" int bde_init(void) {
   int (*const required[])(void) = {bde_internal_load_gauss, bde_internal_load_ivon,       bde_internal_load_lrt,  bde_internal_load_lrt_bwd,
-                                   bde_internal_load_svgd,  bde_internal_load_svgd_fused, bde_internal_load_swag, bde_internal_load_swag_batched};
+                                   bde_internal_load_svgd,  bde_internal_load_svgd_fused, bde_internal_load_swag, bde_internal_load_swag_batched,
+                                   bde_internal_load_embedding, bde_internal_load_topk, bde_internal_load_distill};
   for (auto load : required) {
     const int rc = load();
     if (rc) return rc;

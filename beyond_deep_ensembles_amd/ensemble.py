@@ -10,6 +10,7 @@ result.
 """
 from __future__ import annotations
 
+import math
 from typing import List, Tuple
 
 import torch
@@ -100,6 +101,25 @@ class DeepEnsemble(nn.Module):
                     output.append(predict_closure(model))
             _seek_sampler(optimizer, start, count)                     # where the single-process loop ends
         return torch.stack(output)
+
+    def predict_topk(self, predict_closure, samples, k, *, temperature=1.0, _ops=None):
+        """The ensemble's predictive distribution as a teacher keeps it: ``predict_closure(model)`` returns logits (or
+        log-probabilities) [..., V]; their softmax is averaged over the ``samples`` predictions of ``predict`` and the logarithm of
+        the mean handed to ``topk_logits`` at ``temperature`` -> ``TopLogits(values, indices, rest)``, float32, ready for
+        ``distillation_loss``.  One running [..., V] sum is kept, not the ``samples`` predictions."""
+        from .distill import topk_logits
+        total = None
+
+        def accumulate(model):
+            nonlocal total
+            with torch.no_grad():
+                log_p = torch.log_softmax(predict_closure(model).float(), dim=-1)
+                total = log_p if total is None else torch.logaddexp(total, log_p)
+            return log_p.new_empty(0)
+        if samples < 1:
+            raise ValueError("predict_topk: at least one sample")
+        self.predict(accumulate, samples)
+        return topk_logits(total - math.log(samples), k, temperature=temperature, _ops=_ops)
 
     def predict_distributed(self, predict_closure, samples, process_group=None):
         """MultiX fan-out over the ranks of ``process_group`` (one GPU per rank): every rank evaluates its

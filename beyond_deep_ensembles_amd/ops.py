@@ -41,6 +41,47 @@ def _ptr64(t: torch.Tensor, name: str):
     return t.data_ptr()
 
 
+# element types of the token-model operators (include/bde_hip.h BDE_F32 / BDE_BF16 / BDE_F16)
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX_DTYPES = (torch.int64, torch.int32)
+
+
+def _ptr_typed(t: Optional[torch.Tensor], name: str, dtypes):
+    """Device pointer of a tensor of one of ``dtypes``, last dimension contiguous."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise BdeKernelError(f"{name}: expected a CUDA (HIP) tensor, got device {t.device}; "
+                             "beyond_deep_ensembles_amd has no CPU path")
+    _check_typed(t, name, dtypes)
+    return t.data_ptr()
+
+
+def _check_typed(t, name, dtypes):
+    if t.dtype not in dtypes:
+        raise BdeKernelError(f"{name}: expected {' / '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.dim() > 0 and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise BdeKernelError(f"{name}: last dimension must be contiguous")
+
+
+def _same_device(ref, **others):
+    for name, t in others.items():
+        if t is not None and t.device != ref.device:
+            raise BdeKernelError(f"{name}: on {t.device}, the other operands are on {ref.device}")
+
+
+def _rows(t, name, n, d):
+    """Leading dimension of an [n, d] operand (a single row may have any stride)."""
+    if t.dim() != 2 or tuple(t.shape) != (n, d):
+        raise BdeKernelError(f"{name}: expected shape ({n}, {d}), got {tuple(t.shape)}")
+    return t.stride(0) if n > 1 else d
+
+
+def _flat(t, name, n):
+    if t is not None and (tuple(t.shape) != (n,) or not t.is_contiguous()):
+        raise BdeKernelError(f"{name}: expected a contiguous tensor of shape ({n},), got {tuple(t.shape)}")
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -734,3 +775,110 @@ class HipOps:
         _check(self.lib.bde_ivon_update(_ptr(mean), _ptr(momentum), _ptr(prec), _ptr(delta_sum), _ptr(acc_grad),
                                         lam, n_eff, mc, beta1, 1 - beta1, 1 - beta2, 0.5 * (1 - beta2) ** 2,
                                         1 - beta1 ** t, 1 - beta2 ** t, lr, damping, n, _stream()), "bde_ivon_update")
+
+    # ---------------------------------------------------- token models --
+    NOISE = {None: 0, "position": 1, "token": 2}
+
+    @_on_device_of
+    def embedding_fwd(self, tokens, weight, out, rho=None, noise=None, eps=None, seed=0, stream_id=0, scale=1.0, padding_idx=-1):
+        """out [N, D] = scale * (weight[t] + softplus(rho[t]) * noise) for tokens [N] (bde_embedding_fwd)."""
+        v, d = weight.shape
+        n = tokens.numel()
+        _flat(tokens, "tokens", n)
+        _same_device(weight, tokens=tokens, out=out, rho=rho, eps=eps)
+        if _rows(out, "out", n, d) != d:
+            raise BdeKernelError("embedding_fwd: out must be contiguous")
+        ldw, ldr = _rows(weight, "weight", v, d), 0 if rho is None else _rows(rho, "rho", v, d)
+        lde = 0 if eps is None else _rows(eps, "eps", v if noise == "token" else n, d)
+        f = tuple(DTYPE_CODES)
+        _check(self.lib.bde_embedding_fwd(_ptr_typed(weight, "weight", f), DTYPE_CODES[weight.dtype], ldw, _ptr(rho, "rho"), ldr,
+                                          _ptr_typed(tokens, "tokens", _INDEX_DTYPES), int(tokens.dtype == torch.int64),
+                                          _ptr(eps, "eps"), lde, self.NOISE[noise], seed, stream_id, scale, padding_idx,
+                                          _ptr_typed(out, "out", f), DTYPE_CODES[out.dtype], n, v, d, _stream()), "bde_embedding_fwd")
+
+    @_on_device_of
+    def embedding_bwd(self, g, tokens, g_weight, rho=None, g_rho=None, noise=None, eps=None, seed=0, stream_id=0, scale=1.0,
+                      padding_idx=-1):
+        """g_weight / g_rho [V, D] (overwritten) from g [N, D] (bde_embedding_bwd); with ``rho`` None the noise does not matter."""
+        v, d = g_weight.shape
+        n = tokens.numel()
+        _flat(tokens, "tokens", n)
+        _same_device(g, tokens=tokens, g_weight=g_weight, rho=rho, g_rho=g_rho, eps=eps)
+        if rho is None:
+            noise, eps = None, None
+        ldg = _rows(g, "g", n, d)
+        if _rows(g_weight, "g_weight", v, d) != d or (g_rho is not None and _rows(g_rho, "g_rho", v, d) != d):
+            raise BdeKernelError("embedding_bwd: the gradients must be contiguous")
+        ldr = 0 if rho is None else _rows(rho, "rho", v, d)
+        lde = 0 if eps is None else _rows(eps, "eps", v if noise == "token" else n, d)
+        nbytes = int(self.lib.bde_embedding_bwd_ws_bytes(n, d, self.NOISE[noise]))
+        if nbytes == 0:
+            raise BdeKernelError(f"embedding_bwd: unsupported size N={n}, D={d}")
+        ws = torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=g.device)
+        f = tuple(DTYPE_CODES)
+        _check(self.lib.bde_embedding_bwd(_ptr_typed(g, "g", f), DTYPE_CODES[g.dtype], ldg, _ptr_typed(tokens, "tokens", _INDEX_DTYPES),
+                                          int(tokens.dtype == torch.int64), _ptr(rho, "rho"), ldr, _ptr(eps, "eps"), lde,
+                                          self.NOISE[noise], seed, stream_id, scale, padding_idx,
+                                          _ptr_typed(g_weight, "g_weight", f), DTYPE_CODES[g_weight.dtype], _ptr(g_rho, "g_rho"),
+                                          n, v, d, _ptr(ws), 4 * ws.numel(), _stream()), "bde_embedding_bwd")
+
+    @_on_device_of
+    def topk_logits(self, logits, k, values, indices, rest=None, temperature=1.0):
+        """The k largest of every row of logits [N, V] with their classes and the log-sum of the others (bde_topk_logits)."""
+        n, v = logits.shape
+        _same_device(logits, values=values, indices=indices, rest=rest)
+        ldz = _rows(logits, "logits", n, v)
+        if _rows(values, "values", n, k) != k or _rows(indices, "indices", n, k) != k or values.dtype != logits.dtype:
+            raise BdeKernelError("topk_logits: values (of the logits' type) and indices must be contiguous [N, k]")
+        _flat(rest, "rest", n)
+        f = tuple(DTYPE_CODES)
+        _check(self.lib.bde_topk_logits(_ptr_typed(logits, "logits", f), DTYPE_CODES[logits.dtype], ldz, temperature, n, v, k,
+                                        _ptr_typed(values, "values", f), _ptr_typed(indices, "indices", (torch.int64,)),
+                                        _ptr(rest, "rest"), _stream()), "bde_topk_logits")
+
+    def _distill_teacher(self, logits, values, indices, rest, weight):
+        n, v = logits.shape
+        k = values.shape[-1]
+        _same_device(logits, values=values, indices=indices, rest=rest, weight=weight)
+        if _rows(values, "values", n, k) != k or _rows(indices, "indices", n, k) != k:
+            raise BdeKernelError("distill: values and indices must be contiguous [N, K]")
+        _flat(rest, "rest", n)
+        _flat(weight, "weight", n)
+        f = tuple(DTYPE_CODES)
+        return (_ptr_typed(logits, "logits", f), DTYPE_CODES[logits.dtype], _rows(logits, "logits", n, v), _ptr_typed(values, "values", f),
+                DTYPE_CODES[values.dtype], _ptr_typed(indices, "indices", _INDEX_DTYPES), int(indices.dtype == torch.int64),
+                _ptr(rest, "rest"), _ptr(weight, "weight")), (n, v, k)
+
+    REDUCTION = {"none": 0, "sum": 1, "mean": 2}
+
+    def _distill_grad(self, grad, logits):
+        if grad.dtype != logits.dtype or _rows(grad, "grad", *logits.shape) != logits.shape[1]:
+            raise BdeKernelError("distill: grad must be contiguous, of the logits' shape and type")
+        _same_device(logits, grad=grad)
+        return _ptr_typed(grad, "grad", tuple(DTYPE_CODES))
+
+    @_on_device_of
+    def distill_fwd(self, logits, values, indices, rest, weight, loss_rows, loss=None, grad=None, inv_weight=None, reduction="mean",
+                    scale=1.0, temperature=1.0):
+        """Losses of the rows, their reduction and (with ``grad``) the gradient in the same pass (bde_distill_fwd)."""
+        teacher, (n, v, k) = self._distill_teacher(logits, values, indices, rest, weight)
+        _flat(loss_rows, "loss_rows", n)
+        _same_device(logits, loss_rows=loss_rows, loss=loss, inv_weight=inv_weight)
+        g = None if grad is None else self._distill_grad(grad, logits)
+        _check(self.lib.bde_distill_fwd(*teacher, self.REDUCTION[reduction], scale, temperature, n, v, k, _ptr(loss_rows, "loss_rows"),
+                                        _ptr(loss, "loss"), g, _ptr(inv_weight, "inv_weight"), _stream()), "bde_distill_fwd")
+
+    @_on_device_of
+    def distill_bwd(self, logits, values, indices, rest, weight, upstream, grad, inv_weight=None, mean=False, skip_if_one=False,
+                    scale=1.0, temperature=1.0):
+        """grad for a given d objective / d loss: one value or one per row (bde_distill_bwd)."""
+        teacher, (n, v, k) = self._distill_teacher(logits, values, indices, rest, weight)
+        per_row = upstream.dim() == 1
+        if per_row:
+            _flat(upstream, "upstream", n)
+        elif upstream.numel() != 1:
+            raise BdeKernelError("distill_bwd: upstream must hold one value, or one per row")
+        _same_device(logits, upstream=upstream, inv_weight=inv_weight)
+        _check(self.lib.bde_distill_bwd(*teacher, _ptr(inv_weight, "inv_weight"), int(mean), scale, temperature,
+                                        _ptr(upstream, "upstream"), int(per_row), int(skip_if_one), n, v, k,
+                                        self._distill_grad(grad, logits), _stream()), "bde_distill_bwd")

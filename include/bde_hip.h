@@ -40,6 +40,13 @@ extern "C" {
 #define BDE_GMAT_DOUBLES 257    /* bde_svgd_gram_finish: 16 x 16 Gram matrix (row-major, padded) + its padded M */
 #define BDE_MAX_RANK 256       /* SWAG: deviation_samples K <= 256           */
 #define BDE_MAX_BATCH 32       /* SWAG batched sampling: S <= 32 per call    */
+/* element types of the token-model operators (everything else is fp32) */
+#define BDE_F32 0
+#define BDE_BF16 1
+#define BDE_F16 2
+#define BDE_EMBEDDING_MAX_TOKENS (1 << 28)
+#define BDE_EMBEDDING_MAX_ROWS (1 << 24)
+#define BDE_EMBEDDING_MAX_DIM 16384
 
 /* Library/ABI version (major*10000 + minor*100 + patch). */
 int bde_version(void);
@@ -508,6 +515,62 @@ int bde_ivon_sample(const float* mean, const float* prec, const float* eps, uint
 int bde_ivon_update(float* mean, float* momentum, float* prec, const float* delta_sum, const float* acc_grad,
                     float lam, float n_eff, float mc, float beta1, float omb1, float omb2, float c2,
                     float bc1, float bc2, float lr, float damping, int64_t n, void* stream);
+
+/* ------------------------------------------------------- token models --
+ * The two ends of a text model trained with this library (no reference counterpart: its text models take both from
+ * torch): the embedding of the input tokens, plain or mean-field Gaussian, and the distillation of a teacher -- an
+ * ensemble's predictive distribution -- kept as the top logits of each row.  Arithmetic is fp32; bf16 / fp16 operands are
+ * read as they are and results are rounded to their type once.  `ld*` count elements; rows need no alignment beyond their
+ * element's, except the gradients of tables (16 bytes).
+ *
+ * Scaled embedding lookup, out [N, D]:
+ *   noise 0 (rho, eps NULL)   out_i = scale * weight[t_i]
+ *   noise 1 (by position)     out_i = scale * (weight[t_i] + softplus(rho[t_i]) * eps_i),        eps [N, ldeps]
+ *   noise 2 (by token)        out_i = scale * (weight[t_i] + softplus(rho[t_i]) * eps[t_i]),     eps [V, ldeps]
+ * eps NULL: Philox, element i * D + d (1) or t * D + d (2) of stream `stream_id` -- noise 2 then reads the draw that
+ * bde_gauss_draw_fwd makes of the whole table.  tokens: int64 (tokens64 != 0) or int32.  A position holding `padding` (-1:
+ * none) gets no noise and no gradient; one holding a token outside [0, V) gets a row of NaN and no gradient.
+ * Types: weight and out equal, or an fp32 weight with any out; fp32 weight with noise. */
+int bde_embedding_fwd(const void* weight, int weight_dtype, int64_t ldw, const float* rho, int64_t ldrho, const void* tokens,
+                      int tokens64, const float* eps, int64_t ldeps, int noise, uint64_t seed, uint64_t stream_id, float scale,
+                      int64_t padding, void* out, int out_dtype, int64_t N, int64_t V, int64_t D, void* stream);
+/* Its backward for g [N, ldg]: g_weight [V, D] = scale * sum of the rows of g per token, and with noise
+ * g_rho [V, D] = scale * sigmoid(rho) * sum of g * eps; both OVERWRITTEN whole (rows of absent tokens are zero).  The
+ * positions are sorted by token and added in their order: bit-reproducible.  ws: bde_embedding_bwd_ws_bytes(N, D, noise). */
+size_t bde_embedding_bwd_ws_bytes(int64_t N, int64_t D, int noise);
+int bde_embedding_bwd(const void* g, int g_dtype, int64_t ldg, const void* tokens, int tokens64, const float* rho, int64_t ldrho,
+                      const float* eps, int64_t ldeps, int noise, uint64_t seed, uint64_t stream_id, float scale, int64_t padding,
+                      void* g_weight, int weight_dtype, float* g_rho, int64_t N, int64_t V, int64_t D, void* ws, size_t ws_bytes,
+                      void* stream);
+
+/* A teacher's top logits: per row of logits [N, ldz] the K largest values (their own type, falling order, the lower class
+ * ahead among equals; NaN counts as larger than any number) with their classes, and
+ *   rest = log sum_{classes not selected} exp(logit / temperature)           (NULL: not computed; -inf when K == V).
+ * Limits (bde_topk_limits): V <= 262,144, K <= 256. */
+int bde_topk_limits(int* max_classes, int* max_k);
+int bde_topk_logits(const void* logits, int dtype, int64_t ldz, float temperature, int N, int V, int K, void* values,
+                    int64_t* indices, float* rest, void* stream);
+
+/* Distillation from those: with p_j, r = softmax over (values / temperature, rest), q = softmax(logits / temperature) and
+ * Q = sum of q over the classes not listed,
+ *   loss_i = scale * weight_i * ( sum_j p_j (log p_j - log q_{v_j}) + r (log r - log Q) ).
+ * rest NULL: the list is all there is (r = 0); weight NULL: 1.  Entries with an index outside [0, V) are not used; entries of
+ * one class add up; a row of weight 0, or whose teacher says nothing (no entry, rest -inf), has loss 0 and gradient 0
+ * whatever its logits hold.  reduction 0: loss_rows [N] only; 1: *loss = their sum; 2: *loss = their sum / sum of the weights
+ * (N without weights; 0 when that sum is 0), inv_weight (one float, with weights) receives 1 / that sum for bde_distill_bwd.
+ * grad (may be NULL) [N, V] contiguous, the logits' type: d (sum of the rows' losses as reduced) / d logits, in the same pass
+ * over the logits.  Limits (bde_distill_limits): V <= 262,144, K <= 1,024. */
+int bde_distill_limits(int* max_classes, int* max_entries);
+int bde_distill_fwd(const void* logits, int dtype, int64_t ldz, const void* values, int values_dtype, const void* indices,
+                    int indices64, const float* rest, const float* weight, int reduction, float scale, float temperature, int N,
+                    int V, int K, float* loss_rows, float* loss, void* grad, float* inv_weight, void* stream);
+/* The gradient for a given d objective / d loss: upstream [N] (upstream_stride 1) or one value for all rows (0); rows whose
+ * upstream value is 0 get zeros.  skip_if_one != 0: rows whose value is exactly 1 are left untouched -- `grad` then holds what
+ * bde_distill_fwd wrote, which is bit for bit what this call would write. */
+int bde_distill_bwd(const void* logits, int dtype, int64_t ldz, const void* values, int values_dtype, const void* indices,
+                    int indices64, const float* rest, const float* weight, const float* inv_weight, int mean, float scale,
+                    float temperature, const float* upstream, int64_t upstream_stride, int skip_if_one, int N, int V, int K,
+                    void* grad, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,7 +17,7 @@ from . import build as B
 
 
 ALL = ["version.hip", "swag.hip", "swag_batched.hip", "svgd.hip", "svgd_small.hip", "svgd_fused.hip", "gauss.hip", "ivon.hip",
-       "lrt.hip", "lrt_bwd.hip", "conv_lrt.hip", "conv_lrt_bwd.hip"]
+       "lrt.hip", "lrt_bwd.hip", "conv_lrt.hip", "conv_lrt_bwd.hip", "embedding.hip", "topk.hip", "distill.hip"]
 
 
 class _Shadows:
@@ -148,7 +148,18 @@ def emulated(sources, defines=()):
             raise ops_mod.BdeKernelError(f"{name}: expected a float64 CPU tensor on the model, got {t.dtype} on {t.device}")
         return shadows.ptr(t)
 
+    real_typed = ops_mod._ptr_typed
+
+    def ptr_typed(t, name, dtypes):
+        if t is None:
+            return None
+        if t.is_cuda:
+            raise AssertionError("emulated HipOps takes CPU tensors")
+        ops_mod._check_typed(t, name, dtypes)
+        return shadows.ptr(t)
+
     ops_mod._ptr, ops_mod._check, ops_mod._stream, ops_mod._ptr64 = ptr, check, lambda: None, ptr64
+    ops_mod._ptr_typed = ptr_typed
     real_device, real_sync = torch.cuda.device, torch.cuda.synchronize
     torch.cuda.device = lambda dev: contextlib.nullcontext()          # "the output's device is current": nothing to do
     torch.cuda.synchronize = lambda *a, **k: None                     # every emulated launch has finished when it returns
@@ -158,3 +169,4 @@ def emulated(sources, defines=()):
         shadows.land()
         torch.cuda.device, torch.cuda.synchronize = real_device, real_sync
         ops_mod._ptr, ops_mod._check, ops_mod._stream, ops_mod._ptr64 = real_ptr, real_check, real_stream, real_ptr64
+        ops_mod._ptr_typed = real_typed

@@ -21,6 +21,16 @@
 #include <thread>
 #include <vector>
 
+// fp32 -> bf16, round to nearest even (the host's runtime library may lack it)
+extern "C" __attribute__((weak, visibility("hidden"))) __bf16 __truncsfbf2(float x) {
+  uint32_t b;
+  std::memcpy(&b, &x, 4);
+  const uint16_t r = x != x ? static_cast<uint16_t>((b >> 16) | 0x40u) : static_cast<uint16_t>((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
+  __bf16 out;
+  std::memcpy(&out, &r, 2);
+  return out;
+}
+
 namespace hip_emu {
 
 thread_local Lane* cur = nullptr;

@@ -167,6 +167,12 @@ inline void global_load_lds(const __attribute__((address_space(1))) void* src, _
   dma_request((const void*)src, base + offset + cur->lane * bytes, bytes);
 }
 
+// v_exp_f32: results below the smallest normal number are zero
+inline float exp2_flushed(float x) {
+  const float r = std::exp2(x);
+  return r < 1.17549435e-38f ? 0.0f : r;
+}
+
 inline uint32_t bitop3(uint32_t a, uint32_t b, uint32_t c, uint32_t table) {
   uint32_t out = 0;
   for (int bit = 0; bit < 32; ++bit) {
@@ -199,6 +205,7 @@ inline void __syncthreads() { hip_emu::block_sync(); }
 #define __builtin_amdgcn_fence(...) ((void)0)
 #define __builtin_amdgcn_sqrtf(x) std::sqrt(static_cast<float>(x))
 #define __builtin_amdgcn_logf(x) std::log2(static_cast<float>(x))
+#define __builtin_amdgcn_exp2f(x) hip_emu::exp2_flushed(x)
 #define __builtin_amdgcn_rcpf(x) (1.0f / static_cast<float>(x))
 #define __builtin_amdgcn_cosf(x) static_cast<float>(std::cos(6.283185307179586 * static_cast<double>(x)))
 #define __builtin_amdgcn_sinf(x) static_cast<float>(std::sin(6.283185307179586 * static_cast<double>(x)))
@@ -227,5 +234,8 @@ inline void atomic_store(T* p, T v) { __atomic_store(p, &v, __ATOMIC_SEQ_CST); }
 template <typename T>
 inline T atomic_load(const T* p) { T v; __atomic_load(const_cast<T*>(p), &v, __ATOMIC_SEQ_CST); return v; }
 }  // namespace hip_emu
+inline int atomicAdd(int* p, int v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }
+inline uint32_t atomicOr(uint32_t* p, uint32_t v) { return __atomic_fetch_or(p, v, __ATOMIC_SEQ_CST); }
+inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 #define __hip_atomic_store(p, v, order, scope) hip_emu::atomic_store((p), (v))
 #define __hip_atomic_load(p, order, scope) hip_emu::atomic_load((p))

@@ -21,6 +21,7 @@ BEGIN, END = "<!-- KERNEL-TABLE:BEGIN (tools/kernel_table.py --write) -->", "<!-
 # device status keys
 R3 = "yes -- green in the driver's r03 suite (GPUTEST_r03), source unchanged since"
 R4B = "yes -- green in builder calls r4b/r4c (profiles/r04_pytest_gpu_call_{b,c}.log) after its last change"
+TOK = "yes -- green with `tests/test_token_ops.py` (`-m gpu`)"
 NEVER = ("**no** -- changed after the last GPU call (pool closed since round 4); runs on the CPU model only; NOT a default path "
          "until `device_verified.json` records a green device run of these sources (§0)")
 
@@ -107,6 +108,16 @@ ROWS = {
     # ---- iVON
     "ivon_sample_kernel": ("`ivorn.py:102-115`", "`20·D` B", "0.0737 ms = 6.48 TB/s (0.81); r4", R3, "`test_ivon_golden_bit_exact`"),
     "ivon_update_kernel": ("`ivorn.py:66-89`", "`32·D` B", "0.1158 ms = 6.60 TB/s (0.825); r4", R3, "`test_ivon_golden_bit_exact` (bit-exact)"),
+    # ---- token models
+    "embedding_fwd_kernel": ("the lookup, scaling and noise of a token model's first layer (torch's index_select + mul + add)", "rows touched + `N·D` out", "see §5.3", TOK,
+                             "`test_embedding_*`, `test_gaussian_embedding`"),
+    "embedding_sort_kernel": ("positions sorted by token in one launch; zero rows of absent tokens", "`8·N` B + the absent rows", "see §5.3", TOK, "same"),
+    "embedding_sum_kernel": ("the tokens' gradient rows, added in order (torch: atomics)", "`N·D` in, touched rows out", "see §5.3", TOK, "same"),
+    "embedding_join_kernel": ("runs that cross a piece of the sorted list", "latency", "see §5.3", TOK, "`test_embedding_token_patterns`"),
+    "topk_logits_kernel": ("a teacher's k largest logits, their classes and the log-sum of the rest", "`N·V` read once", "see §5.3", TOK, "`test_topk_*`"),
+    "distill_topk_kernel": ("distillation loss over a teacher's top logits and its gradient in one pass", "`N·V` read once, written once", "see §5.3", TOK, "`test_distill_*`"),
+    "distill_inv_weight_kernel": ("1 / sum of the rows' weights", "latency", "—", TOK, "`test_distill_reductions_and_upstream_values`"),
+    "distill_sum_kernel": ("the rows' losses → one number, fixed order", "latency", "—", TOK, "same test"),
 }
 
 

@@ -20,7 +20,8 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "beyond_deep_ensembles_amd", "csrc")
 HIPCC = "/opt/rocm/bin/hipcc"
-FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-fno-fast-math", "-I" + os.path.join(ROOT, "include"),
+FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off", "-fno-fast-math", "-Xclang", "-target-feature",
+         "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"),
          "-Rpass-analysis=kernel-resource-usage"]                     # the Makefile's flags + the remark
 
 
