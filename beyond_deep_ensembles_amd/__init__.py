@@ -27,5 +27,6 @@ _LAZY = {
 def __getattr__(name):
     if name in _LAZY:
         import importlib
-        return getattr(importlib.import_module(_LAZY[name], __name__), name)
+        value = globals()[name] = getattr(importlib.import_module(_LAZY[name], __name__), name)     # found directly from now on
+        return value
     raise AttributeError(name)

@@ -205,21 +205,21 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
   }
   if (tid == 0 && hi == a.V) a.header[0] = all;
   __syncthreads();
-  // positions in order: lanes of one token take consecutive places
+  // positions in order: lanes of one token take consecutive places (the lanes that agree with this one on every bit of the
+  // token's number in the bucket: a ballot per bit, whatever the tokens are)
+  const int bits = 32 - __builtin_clz(a.bucket | 1);
   auto place = [&](bool in, int r, int p) {
-    unsigned long long todo = __ballot(in);
-    while (todo) {
-      const int leader = __builtin_ctzll(todo);
-      const int lr = __shfl(r, leader, 64);
-      const unsigned long long m = __ballot(in && r == lr);
-      const int at = mine[lr];
-      if (in && r == lr) {
-        const int to = at + __popcll(m & before);
-        a.order[to] = p;
-        a.key[to] = lo + lr;
-      }
-      if (lane == leader) mine[lr] = at + __popcll(m);
-      todo &= ~m;
+    unsigned long long same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const bool set = (r >> b) & 1;
+      const unsigned long long m = __ballot(set);
+      same &= set ? m : ~m;
+    }
+    const int at = in ? mine[r] : 0, rank = __popcll(same & before);
+    if (in) {
+      a.order[at + rank] = p;
+      a.key[at + rank] = lo + r;
+      if (rank == 0) mine[r] = at + __popcll(same);
     }
   };
   if (fits) {
@@ -232,7 +232,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
       const int p = base + lane;
       int t = p < end ? load_index(a.tokens, a.tokens64, p, a.V) : -1;
       if (t == pad) t = -1;
-      place(t >= lo && t < hi, t - lo, p);
+      const bool in = t >= lo && t < hi;
+      place(in, in ? t - lo : 0, p);
     }
   }
   // rows of tokens that do not occur: zero

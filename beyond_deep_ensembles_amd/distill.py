@@ -12,6 +12,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
+from .lookup import _backend
 from .ops import BdeKernelError, DTYPE_CODES
 
 
@@ -19,13 +20,6 @@ class TopLogits(NamedTuple):
     values: torch.Tensor        # [..., k], the logits' type, falling
     indices: torch.Tensor       # [..., k], int64
     rest: torch.Tensor          # [...], float32: log sum over the other classes of exp(logit / temperature)
-
-
-def _backend(ops):
-    if ops is None:
-        from .algo import _default_ops
-        ops = _default_ops()
-    return ops
 
 
 def _logit_rows(logits, name="logits"):
@@ -53,16 +47,20 @@ def _temperature(t) -> float:
 def topk_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, _ops=None) -> TopLogits:
     """The ``k`` largest logits of every row in falling order (the lower class ahead among equals, a NaN above every number)
     with their classes, and the log-sum of the others at ``temperature``.  Log-probabilities are logits.  No gradient."""
+    temperature = _temperature(temperature)
+    k = int(k)
+    _ops, native = _backend(_ops)
+    if native is not None:
+        return TopLogits(*native.topk_logits(logits, k, temperature))
     rows = _logit_rows(logits.detach())
     n, v = rows.shape
-    k = int(k)
     if not 1 <= k <= min(v, 256) or v > 262144:
         raise BdeKernelError(f"topk_logits: 1 <= k <= min(V, 256) and V <= 262144 supported, got k={k}, V={v}")
     shape = logits.shape[:-1]
     values = torch.empty((n, k), dtype=rows.dtype, device=rows.device)
     indices = torch.empty((n, k), dtype=torch.int64, device=rows.device)
     rest = torch.empty(n, dtype=torch.float32, device=rows.device)
-    _backend(_ops).topk_logits(rows, k, values, indices, rest, temperature=_temperature(temperature))
+    _ops.topk_logits(rows, k, values, indices, rest, temperature=temperature)
     return TopLogits(values.view(shape + (k,)), indices.view(shape + (k,)), rest.view(shape))
 
 
@@ -125,6 +123,9 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction: 'none', 'sum' or 'mean', not {reduction!r}")
     temperature = _temperature(temperature)
+    _ops, native = _backend(_ops)
+    if native is not None:
+        return native.distillation_loss(logits, values, indices, rest, weight, _ops.REDUCTION[reduction], scale, temperature)
     rows = _logit_rows(logits)
     n, v = rows.shape
     lead = tuple(logits.shape[:-1])
@@ -141,5 +142,5 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
         if t is not None and t.requires_grad:
             raise BdeKernelError(f"{name}: the teacher's side and the weights are constants of this loss (no gradient); detach them")
     flat = [_dense(values, (n, k)), _dense(indices, (n, k))] + [None if t is None else _dense(t, (n,)) for t in (rest, weight)]
-    loss = _Distill.apply(rows, *flat, reduction, float(scale), temperature, _backend(_ops))
+    loss = _Distill.apply(rows, *flat, reduction, float(scale), temperature, _ops)
     return loss.view(lead) if reduction == "none" else loss

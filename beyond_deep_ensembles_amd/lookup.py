@@ -17,6 +17,23 @@ from .ops import BdeKernelError, DTYPE_CODES
 from .util import _philox_stream
 
 _TOKEN_TYPES = (torch.int64, torch.int32)
+_layers = None
+_default = None         # the product's one backend, made at the first call that names none
+
+
+def _backend(ops):
+    """(the kernel backend, the C++ nodes of lib/_bde_host.so or None): the nodes (csrc/host_autograd.cpp) are what this module's
+    Python path does, without its interpreter time; they exist for the HIP library only."""
+    global _layers, _default
+    if _layers is None:
+        from . import algo, bbb_layers
+        _layers = (algo, bbb_layers)
+    if ops is None:
+        if _default is None:
+            _default = _layers[0]._default_ops()
+        ops = _default
+    native = _layers[1]._native_nodes(ops)
+    return ops, native if native is not None and hasattr(native, "distillation_loss") else None
 
 
 def _table(tokens, weight, padding_idx, out_dtype, scale):
@@ -89,10 +106,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
 
     The gradient of ``weight`` is dense and leaves out the positions that hold ``padding_idx``.  A token outside [0, V) gives
     a row of NaN and no gradient (the host does not look at the tokens)."""
+    _ops, native = _backend(_ops)
+    if native is not None:
+        return native.embedding(tokens, weight, None, None, 0, 0, 0, scale, padding_idx, out_dtype)
     padding_idx, out_dtype, scale = _table(tokens, weight, padding_idx, out_dtype, scale)
-    if _ops is None:
-        from .algo import _default_ops
-        _ops = _default_ops()
     return _Embedding.apply(weight, None, tokens, None, out_dtype, None, 0, 0, scale, padding_idx, _ops)
 
 
@@ -107,9 +124,14 @@ def gaussian_embedding(tokens: torch.Tensor, mean: torch.Tensor, rho: torch.Tens
     ``stream_id`` of ``seed``, a fresh stream per call by default) and generate it again in the backward pass; by token it is
     the noise ``GaussianParameter.sample()`` of that stream has.  Positions that hold ``padding_idx`` have no noise and no
     gradient."""
-    padding_idx, out_dtype, scale = _table(tokens, mean, padding_idx, out_dtype, scale)
     if noise not in ("position", "token"):
         raise ValueError(f"noise: 'position' or 'token', not {noise!r}")
+    if eps is None and stream_id is None:
+        stream_id = next(_philox_stream)
+    _ops, native = _backend(_ops)
+    if native is not None:
+        return native.embedding(tokens, mean, rho, eps, 1 if noise == "position" else 2, int(seed), int(stream_id or 0), scale, padding_idx, out_dtype)
+    padding_idx, out_dtype, scale = _table(tokens, mean, padding_idx, out_dtype, scale)
     if mean.dtype != torch.float32 or rho.dtype != torch.float32 or rho.shape != mean.shape or rho.device != mean.device:
         raise BdeKernelError("gaussian_embedding: mean and rho must be float32 tensors of one shape and device")
     n, (v, d) = tokens.numel(), mean.shape
@@ -121,11 +143,6 @@ def gaussian_embedding(tokens: torch.Tensor, mean: torch.Tensor, rho: torch.Tens
         if eps.requires_grad:
             raise BdeKernelError("eps: the noise is a constant of this operator (no gradient); detach it")
         eps = _row_major(eps.reshape(v if noise == "token" else n, d))
-    elif stream_id is None:
-        stream_id = next(_philox_stream)
-    if _ops is None:
-        from .algo import _default_ops
-        _ops = _default_ops()
     return _Embedding.apply(mean, rho, tokens, eps, out_dtype, noise, int(seed), int(stream_id or 0), scale, padding_idx, _ops)
 
 

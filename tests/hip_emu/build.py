@@ -138,6 +138,8 @@ def build_host_nodes(sources):
     old_stream = "void* current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }"
     assert old_stream in text and "t.is_cuda() &&" in text and "#include <c10/hip/HIPStream.h>\n" in text
     text = text.replace(old_stream, "void* current_stream(const at::Tensor&) { return nullptr; }")
+    old_capture = next(ln for ln in text.splitlines() if ln.startswith("bool stream_capturing(void* stream)"))
+    text = text.replace(old_capture, "bool stream_capturing(void*) { return false; }")
     text = text.replace("t.is_cuda() &&", "!t.is_cuda() &&").replace("#include <c10/hip/HIPStream.h>\n", "")
     text = text.replace('#include "../../include/bde_hip.h"', f'#include "{os.path.join(ROOT, "include", "bde_hip.h")}"')
     text += "\nPYBIND11_MODULE(_bde_host_emu, m) { bind_autograd_nodes(m); }\n"

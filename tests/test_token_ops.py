@@ -17,15 +17,16 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 NAMES = {F32: "f32", BF16: "bf16", F16: "f16"}
 
 
-@pytest.fixture(params=["emu", pytest.param("hip", marks=pytest.mark.gpu)])
+@pytest.fixture(params=["emu", "emu_python", pytest.param("hip", marks=pytest.mark.gpu)])
 def backend(request, monkeypatch):
-    if request.param == "emu":
+    if request.param != "hip":
         from tests.hip_emu import build, emu_ops
         if not build.available():
             pytest.skip("no host clang / HIP headers to build the CPU model with")
-        # the C++ autograd nodes are there too, compiled over the model (lib/_bde_host.so binds the device library)
+        # "emu": through the C++ autograd nodes, compiled over the model (lib/_bde_host.so binds the device library);
+        # "emu_python": through the Python ones
         import beyond_deep_ensembles_amd.bbb_layers as L
-        native = build.load_host_nodes(emu_ops.ALL)
+        native = build.load_host_nodes(emu_ops.ALL) if request.param == "emu" else None
         monkeypatch.setattr(L, "_native_nodes", lambda ops: native)
         with emu_ops.emulated(emu_ops.ALL) as ops:
             yield ops, torch.device("cpu")
