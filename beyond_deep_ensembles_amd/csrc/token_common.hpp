@@ -122,18 +122,32 @@ __device__ __forceinline__ float wave_all_sum(float x) {
 __device__ __forceinline__ float wave_all_max(float x) {
   return wave_all(x, [](float a, float b) { return fmaxf(a, b); });
 }
-// The same over a workgroup of NT threads: one value per wave in `slots` (>= NT / 64 floats, not used by a reduction still
-// being read), ONE barrier; every wave sums the slots in the same order.
+// A row is handled by NT threads: a workgroup of its own, or -- rows that fit one wave -- one of the four waves of a workgroup
+// (a launch of one-wave workgroups is bound by their dispatch).  What the lanes of a wave exchange through LDS needs no barrier,
+// only the wait for the LDS operations.
+template <int NT>
+constexpr int kRowsPerGroup = NT == 64 ? 4 : 1;
+template <int NT>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (NT == 64) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+// The reductions over a row's NT threads: one value per wave in `slots` (>= NT / 64 floats, not used by a reduction still being
+// read), ONE barrier; every wave sums the slots in the same order.
 template <int NT, typename F>
-__device__ __forceinline__ float block_all(float x, float* slots, F f) {
+__device__ __forceinline__ float row_all(float x, float* slots, F f) {
   constexpr int W = NT / 64;
   x = wave_all(x, f);
   if constexpr (W == 1) {
-    __syncthreads();               // what the caller wrote to LDS before is visible, whatever NT is
+    row_sync<NT>();                // what the caller wrote to LDS before is visible, whatever NT is
     return x;
   } else {
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = x;
-    __syncthreads();
+    row_sync<NT>();
     float r = slots[0];
 #pragma unroll
     for (int i = 1; i < W; ++i) r = f(r, slots[i]);
@@ -141,12 +155,12 @@ __device__ __forceinline__ float block_all(float x, float* slots, F f) {
   }
 }
 template <int NT>
-__device__ __forceinline__ float block_all_sum(float x, float* slots) {
-  return block_all<NT>(x, slots, [](float a, float b) { return a + b; });
+__device__ __forceinline__ float row_all_sum(float x, float* slots) {
+  return row_all<NT>(x, slots, [](float a, float b) { return a + b; });
 }
 template <int NT>
-__device__ __forceinline__ float block_all_max(float x, float* slots) {
-  return block_all<NT>(x, slots, [](float a, float b) { return fmaxf(a, b); });
+__device__ __forceinline__ float row_all_max(float x, float* slots) {
+  return row_all<NT>(x, slots, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // a token / class index of either width; -1 where it is outside [0, limit)

@@ -43,51 +43,58 @@ __device__ __forceinline__ uint64_t candidate(uint32_t key, int v) {
 }
 
 template <int NT>
-__device__ __forceinline__ int block_count(int n, int* slots) {
+__device__ __forceinline__ int row_count(int n, int* slots) {
   constexpr int W = NT / 64;
   n = static_cast<int>(wave_all_sum(static_cast<float>(n)));      // <= 2^24: exact
-  __syncthreads();                                                // the slots' last readers are done
+  row_sync<NT>();                                                 // the slots' last readers are done
+  if constexpr (W == 1) return n;
   if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = n;
-  __syncthreads();
+  row_sync<NT>();
   int r = 0;
 #pragma unroll
   for (int i = 0; i < W; ++i) r += slots[i];
   return r;
 }
 
-// One workgroup of NT threads per row, the row in registers (NV granules of 16 bytes per thread; NV = 0: rows that do not
-// fit, read again from the caches by each phase).
+// NT threads per row: its first NT * NV granules of 16 bytes are kept in registers, what a longer row has
+// beyond them is read again (from the caches) by the second pass.
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
-  constexpr int GN = Granule<T>::N, W = NT / 64;
-  constexpr int kCap = NT < 1024 ? 1024 : 2048;      // entries of the candidate list
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63;
+__global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(TopkArgs a) {
+  constexpr int GN = Granule<T>::N, W = NT / 64, ROWS = kRowsPerGroup<NT>;
+  constexpr int kCap = NT == 64 ? 128 : 1024;        // entries of the candidate list
+  const int row_of_group = ROWS > 1 ? __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / NT) : 0;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + row_of_group;
+  if (ROWS > 1 && row >= a.N) return;                // (waves that share a workgroup share nothing else)
+  const int tid = static_cast<int>(threadIdx.x) % NT, lane = tid & 63;
+  const int wave_first = __builtin_amdgcn_readfirstlane(tid);       // a wave whose granules all lie behind the row skips them
   const RowView<T> z(static_cast<const T*>(a.z) + row * a.ldz, a.V);
-  __shared__ uint64_t cand[kCap];
-  __shared__ int hits[kCap];
-  __shared__ uint32_t maxima[NT];
-  __shared__ float slots[2 * W];
-  __shared__ int counts[W];
-  __shared__ uint32_t bound;
-  __shared__ int n_hit, n_cand;
+  __shared__ uint64_t cand_[ROWS][kCap];
+  __shared__ int hits_[ROWS][kCap];
+  __shared__ uint32_t maxima_[ROWS][NT];
+  __shared__ float slots_[ROWS][2 * W];
+  __shared__ int counts_[ROWS][W];
+  __shared__ uint32_t bound_[ROWS];
+  __shared__ int n_hit_[ROWS], n_cand_[ROWS];
+  uint64_t* const cand = cand_[row_of_group];
+  int *const hits = hits_[row_of_group], *const counts = counts_[row_of_group];
+  uint32_t* const maxima = maxima_[row_of_group];
+  float* const slots = slots_[row_of_group];
+  uint32_t& bound = bound_[row_of_group];
+  int &n_hit = n_hit_[row_of_group], &n_cand = n_cand_[row_of_group];
 
-  u32x4 reg[NV > 0 ? NV : 1];
-  if constexpr (NV > 0) {
+  u32x4 reg[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) reg[j] = z.load(tid + j * NT);
-  }
+  for (int j = 0; j < NV; ++j)
+    if (wave_first + j * NT < z.granules) reg[j] = z.load(tid + j * NT);
   // f(granule, its number) for this thread's granules
   auto each = [&](auto f) {
-    if constexpr (NV > 0) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        stay_packed(reg[j]);
-        f(reg[j], tid + j * NT);
-      }
-    } else {
-      for (int g = tid; g < z.granules; g += NT) f(z.load(g), g);
+    for (int j = 0; j < NV; ++j) {
+      if (wave_first + j * NT >= z.granules) continue;
+      stay_packed(reg[j]);
+      f(reg[j], tid + j * NT);
     }
+    for (int g = tid + NV * NT; g < z.granules; g += NT) f(z.load(g), g);
   };
   float best = neg_inf();
   each([&](const u32x4& x, int) {
@@ -96,7 +103,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
   });
   maxima[tid] = order_key(best);
   if (tid == 0) n_hit = n_cand = 0;
-  __syncthreads();
+  row_sync<NT>();
   // wave 0: a bound that at least k of the NT maxima reach and not many more (bisection over the keys, counts by ballot)
   if (tid < 64) {
     uint32_t lo = kKeyNegInf;
@@ -127,7 +134,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
     }
     if (lane == 0) bound = lo;
   }
-  __syncthreads();
+  row_sync<NT>();
   const float c = a.inv_tau * kLog2e;
   float least = order_value(bound);                     // (keys between two floats' keys do not exist)
   float ref = least - least == 0.0f ? least : 0.0f;
@@ -150,7 +157,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
       if (at < kCap) hits[at] = g;
     }
   });
-  __syncthreads();
+  row_sync<NT>();
   if (n_hit <= kCap) {
     for (int q = tid; q < n_hit; q += NT) {
       const int e0 = z.first(hits[q]);
@@ -164,7 +171,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
       }
     }
   }
-  __syncthreads();
+  row_sync<NT>();
   int n = n_hit <= kCap ? n_cand : kCap + 1;
   if (n > kCap) {
     // Too many elements reach the bound (they are equal, or nearly all of the row is): the k-th largest key itself, then the
@@ -181,7 +188,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
           m += (v >= 0 && v < a.V && (k > key || (k == key && v <= v_last))) ? 1 : 0;
         }
       }
-      return block_count<NT>(m, counts);
+      return row_count<NT>(m, counts);
     };
     uint32_t key = bound;
     if (count(key, -1) >= a.K) {
@@ -199,9 +206,9 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
       if (count(key, mid) >= a.K) v_hi = mid;
       else v_lo = mid;
     }
-    __syncthreads();
+    row_sync<NT>();
     if (tid == 0) n_cand = 0;
-    __syncthreads();
+    row_sync<NT>();
     least = key == 0xFFFFFFFFu ? __builtin_nanf("") : order_value(key);
     ref = least - least == 0.0f ? least : 0.0f;
     others = 0.0f;
@@ -220,11 +227,11 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
       }
       others += part;
     }
-    __syncthreads();
+    row_sync<NT>();
     n = a.K;
   }
   // rank by counting; what is not selected goes back to the list's front in the order of its rank
-  constexpr int kMine = kCap / NT;
+  constexpr int kMine = (kCap + NT - 1) / NT;
   uint64_t mine[kMine];
   int rank[kMine];
 #pragma unroll
@@ -235,7 +242,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
     if (i < n)
       for (int j = 0; j < n; ++j) rank[q] += cand[j] > mine[q] ? 1 : 0;
   }
-  others = block_all_sum<NT>(others, slots);   // (its barrier: the list has been read)
+  others = row_all_sum<NT>(others, slots);   // (its barrier: the list has been read)
 #pragma unroll
   for (int q = 0; q < kMine; ++q) {
     if (tid + q * NT >= n) continue;
@@ -248,7 +255,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
     }
   }
   if (!a.rest) return;
-  __syncthreads();
+  row_sync<NT>();
   // the candidates left over, relative to the largest of them
   const int left = n - a.K;
   float more = 0.0f, top = 0.0f;
@@ -260,7 +267,7 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
       more += exp2_hw(((key == 0xFFFFFFFFu ? __builtin_nanf("") : order_value(key)) - top) * c);
     }
   }
-  more = block_all_sum<NT>(more, slots + W);
+  more = row_all_sum<NT>(more, slots + W);
   if (tid == 0) {
     float r = neg_inf();
     if (left > 0 && more != 0.0f)              // ref <= top: the others' sum relative to top
@@ -273,23 +280,28 @@ __global__ __launch_bounds__(NT) void topk_logits_kernel(TopkArgs a) {
 
 template <typename T, int NT, int NV>
 static int topk_launch(const TopkArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((topk_logits_kernel<T, NT, NV>), dim3(a.N), dim3(NT), 0, s, a);
+  constexpr int ROWS = kRowsPerGroup<NT>;
+  hipLaunchKernelGGL((topk_logits_kernel<T, NT, NV>), dim3((a.N + ROWS - 1) / ROWS), dim3(NT * ROWS), 0, s, a);
   return to_err(hipGetLastError());
 }
-// Workgroup and registers by the granules of a row, as distill.hip; the small workgroups only while k stays well below their
-// number of threads (the bound comes from the threads' maxima), or while the whole row fits the candidate list.
+// Threads and registers by the granules of a row, as distill.hip: as few waves as hold the row, four to eight granules a thread.
+// The bound comes from the threads' maxima, so a row gets several times k threads.
+// bf16, k = 64: 32,000 classes 36 us with 512 x 8 for 2,048 rows (47 with 1024 x 4); 131,072 classes 280 us with 1024 x 8 and the
+// row's other half read again, 330 us with 1024 x 16 (one workgroup per CU, whose phases then overlap with no other's).
 template <typename T>
 static int topk_pick(const TopkArgs& a, hipStream_t s) {
   constexpr int GN = Granule<T>::N;
   const bool aligned = aligned16(a.z) && (a.ldz % GN == 0 || a.N == 1);
   const int granules = (a.V + (aligned ? 0 : GN - 1) + GN - 1) / GN;
-  if (granules <= 64 && a.K <= 32) return topk_launch<T, 64, 1>(a, s);
-  if (granules <= 256) return topk_launch<T, 256, 1>(a, s);
-  if (granules <= 1024 && a.K <= 128) return topk_launch<T, 256, 4>(a, s);
-  if (granules <= 4096) return topk_launch<T, 1024, 4>(a, s);
-  if (granules <= 8192) return topk_launch<T, 1024, 8>(a, s);
-  if (granules <= 16384) return topk_launch<T, 1024, 16>(a, s);
-  return topk_launch<T, 1024, 0>(a, s);
+  if (a.K <= 24) {
+    if (granules <= 64) return topk_launch<T, 64, 1>(a, s);
+    if (granules <= 256) return topk_launch<T, 64, 4>(a, s);
+  }
+  if (granules <= 1024) return topk_launch<T, 256, 4>(a, s);
+  if (granules <= 2048) return topk_launch<T, 256, 8>(a, s);
+  if (granules <= 4096) return topk_launch<T, 512, 8>(a, s);
+  if (granules <= 6144) return topk_launch<T, 512, 12>(a, s);
+  return topk_launch<T, 1024, 8>(a, s);
 }
 
 }  // namespace bde

@@ -202,6 +202,7 @@ inline void __syncthreads() { hip_emu::block_sync(); }
 #define __builtin_amdgcn_global_load_lds hip_emu::global_load_lds
 #define __builtin_amdgcn_bitop3_b32 hip_emu::bitop3
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
+#define __builtin_amdgcn_wave_barrier() ((void)0)
 #define __builtin_amdgcn_fence(...) ((void)0)
 #define __builtin_amdgcn_sqrtf(x) std::sqrt(static_cast<float>(x))
 #define __builtin_amdgcn_logf(x) std::log2(static_cast<float>(x))

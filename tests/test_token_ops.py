@@ -420,7 +420,8 @@ def teacher(n, v, k, dtype, seed, tau=1.0):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=lambda t: NAMES[t])
-@pytest.mark.parametrize("n,v,k", [(1, 2, 1), (3, 10, 3), (2, 10, 10), (4, 182, 16), (2, 1000, 64), (2, 4100, 100), (1, 9001, 33), (1, 40000, 7)])
+@pytest.mark.parametrize("n,v,k", [(1, 2, 1), (3, 10, 3), (2, 10, 10), (4, 182, 16), (2, 1000, 64), (2, 2500, 20), (2, 4100, 100), (1, 9001, 33),
+                                   (1, 20001, 3), (1, 40000, 7), (1, 70000, 64)])
 def test_distill_sizes_and_types(backend, n, v, k, dtype):
     tau = 1.0 if v % 3 else 2.0
     z, values, indices, rest = teacher(n, v, k, dtype, v + k, tau)
@@ -464,6 +465,16 @@ def test_distill_lists_with_structure(backend, v, k):
         check_distill(backend, z, values, indices, r, tau=1.5)
     check_distill(backend, z, values.bfloat16(), indices.int(), rest, tau=0.7, reduction="none")
     z[5] = math.nan                                    # (nothing said: not looked at)
+    check_distill(backend, z, values, indices, rest)
+
+
+@pytest.mark.parametrize("v,spike", [(3000, 2900), (20001, 19990), (70000, 69000)])
+def test_distill_rows_that_rise_late(backend, v, spike):
+    """The largest classes lie behind each thread's first granule, so far above it that the provisional reference overflows; and
+    rows whose first granules are masked entirely."""
+    z, values, indices, rest = teacher(2, v, 5, F32, v)
+    z[0, spike:spike + 3] += 150.0
+    z[1, :v // 2] = -math.inf
     check_distill(backend, z, values, indices, rest)
 
 
