@@ -40,7 +40,13 @@ struct EmbedArgs {
   int* key;                // [N] their tokens
   float* part;             // [pieces][2][accumulators][D] sums of the runs that cross a piece's borders
   int piece;
-  int bucket;              // tokens per workgroup of the sort
+  int log_groups, bucket;  // workgroups of the sort (a power of two) and the most tokens one of them owns
+  int chunk;               // > 0: the tokens are dealt out to the sort's workgroups first, this many per workgroup of that
+  int* counts;             // [chunks][groups]
+  int* group_start;        // [groups + 1]
+  int* dealt_p;            // [N] positions by group, in order
+  int* dealt_t;            // [N] their tokens
+  int stream_zeros;        // zero rows are stored past the caches
 };
 
 // VEC consecutive elements as fp32
@@ -88,113 +94,250 @@ __device__ __forceinline__ void noise_vec(uint64_t seed, uint64_t stream_id, int
   }
 }
 
-// 2^log_lanes lanes per row
-template <typename TW, typename TO, int NOISE, int VEC>
+// 2^log_lanes lanes per row, ROWS rows per group of lanes (their loads in flight together)
+template <typename TW, typename TO, int NOISE, int VEC, int ROWS>
 __global__ __launch_bounds__(kBlock) void embedding_fwd_kernel(EmbedArgs a, int log_lanes) {
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) >> log_lanes;
-  if (row >= a.N) return;
+  const int64_t first = ((static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) >> log_lanes) * ROWS;
   const int lanes = 1 << log_lanes, lane = threadIdx.x & (lanes - 1);
-  const int t = load_index(a.tokens, a.tokens64, row, a.V);
-  TO* const out = static_cast<TO*>(a.out) + row * a.D;
-  const float scale = t >= 0 ? a.scale : __builtin_nanf("");
-  const int64_t tr = t >= 0 ? t : 0;
-  const TW* const w = static_cast<const TW*>(a.weight) + tr * a.ldw;
-  const bool noisy = NOISE != kNoiseNone && t != a.padding;
-  const int64_t noise_row = NOISE == kNoisePosition ? row : tr;
-#pragma unroll 4
-  for (int d = lane * VEC; d < a.D; d += lanes * VEC) {
-    float f[VEC];
-    load_vec<TW, VEC>(w + d, f);
-    if constexpr (NOISE != kNoiseNone) {
-      if (noisy) {
-        float r[VEC], e[VEC];
-        load_vec<float, VEC>(a.rho + tr * a.ldrho + d, r);
-        if (a.eps) load_vec<float, VEC>(a.eps + noise_row * a.ldeps + d, e);
-        else noise_vec<VEC>(a.seed, a.stream_id, noise_row * a.D + d, e);
+  int t[ROWS];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] += softplus(r[i]) * e[i];
+  for (int u = 0; u < ROWS; ++u) t[u] = first + u < a.N ? load_index(a.tokens, a.tokens64, first + u, a.V) : -1;
+  for (int d = lane * VEC; d < a.D; d += lanes * VEC) {
+    float f[ROWS][VEC], r[NOISE != kNoiseNone ? ROWS : 1][VEC], e[NOISE != kNoiseNone ? ROWS : 1][VEC];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int64_t row = first + u, tr = t[u] >= 0 ? t[u] : 0;
+      load_vec<TW, VEC>(static_cast<const TW*>(a.weight) + tr * a.ldw + d, f[u]);
+      if constexpr (NOISE != kNoiseNone) {
+        const int64_t noise_row = NOISE == kNoiseToken ? tr : row < a.N ? row : 0;
+        load_vec<float, VEC>(a.rho + tr * a.ldrho + d, r[u]);
+        if (a.eps) load_vec<float, VEC>(a.eps + noise_row * a.ldeps + d, e[u]);
+        else noise_vec<VEC>(a.seed, a.stream_id, noise_row * a.D + d, e[u]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] *= scale;
-    store_vec<TO, VEC>(out + d, f);
+    for (int u = 0; u < ROWS; ++u) {
+      if constexpr (NOISE != kNoiseNone) {
+        if (t[u] != a.padding) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[u][i] += softplus(r[u][i]) * e[u][i];
+        }
+      }
+      const float scale = t[u] >= 0 ? a.scale : __builtin_nanf("");
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[u][i] *= scale;
+      if (first + u < a.N) store_vec<TO, VEC>(static_cast<TO*>(a.out) + (first + u) * a.D + d, f[u]);
+    }
   }
 }
 
 // ---------------------------------------------------------------- gradient --
-// Stable counting sort in ONE launch.  A workgroup owns the tokens [lo, lo + bucket): it reads ALL tokens, counts those of its
-// own range (per wave and token) and those below its range -- the latter is where its part of the sorted list begins, so no
-// scan between workgroups is needed -- and writes its positions in order.  The 16 waves take 16 consecutive parts of the list;
-// a wave keeps the matches of its part in LDS and reads its part again only when they do not fit.  Rows of tokens that do not
-// occur are zero-filled here.
-// Work: (tokens / 64) wave-steps per workgroup, the list comes from L2 after the first reader.
-constexpr int kSortThreads = 1024, kSortWaves = 16, kSortList = 256, kMaxBucket = 512;
+// Stable counting sort in ONE launch.  Workgroup b of a power of two owns the tokens t = b, b + count, b + 2 count, ... (strided,
+// because frequent tokens lie side by side in a vocabulary): it reads ALL tokens, counts its own (per wave and token) and those
+// of the workgroups before it -- which is where its part of the sorted list begins, so no scan between workgroups is needed --
+// and writes its positions, one token after the other, each token's in order.  The 16 waves take 16 consecutive parts of the
+// list; a wave keeps the matches of its part in LDS and reads its part again only when they do not fit.  Rows of tokens that do
+// not occur are zero-filled here.
+// Work: (tokens / 64) wave-steps per workgroup, the list comes from L2 after the first reader; with a large table the zero rows
+// bound the kernel (a stream of stores).
+constexpr int kSortThreads = 1024, kSortWaves = 16, kSortList = 256, kMaxBucket = 512, kMaxDealGroups = 512;
 
-template <typename TW>
-__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs a) {
-  extern __shared__ int hist[];                     // [16][bucket] counts, then where the next one goes
-  __shared__ int list_p[kSortWaves][kSortList];
-  __shared__ uint16_t list_r[kSortWaves][kSortList];
-  __shared__ int sums[kSortWaves], below[kSortWaves], totals[kMaxBucket];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int lo = static_cast<int>(blockIdx.x) * a.bucket, hi = min(a.V, lo + a.bucket), own = hi - lo;
-  for (int i = tid; i < kSortWaves * a.bucket; i += kSortThreads) hist[i] = 0;
+// a token as it lies in memory: looked at when it is used, not when it is loaded
+__device__ __forceinline__ int64_t raw_token(const EmbedArgs& a, int64_t i) {
+  return a.tokens64 ? static_cast<const int64_t*>(a.tokens)[i] : static_cast<const int*>(a.tokens)[i];
+}
+__device__ __forceinline__ bool live_token(const EmbedArgs& a, int64_t raw) {    // false: no gradient
+  const uint32_t lo = static_cast<uint32_t>(raw), hi = static_cast<uint32_t>(static_cast<uint64_t>(raw) >> 32);
+  return hi == 0 && lo < static_cast<uint32_t>(a.V) && lo != static_cast<uint32_t>(a.padding);
+}
+
+// With many tokens the workgroups do not read all of them: two short kernels deal the positions out first (count per chunk and
+// group; then each chunk writes its positions behind those of the chunks before it).  Gradient of a 30,011 x 256
+// fp32 table: 32,768 tokens 35 us without, 39 with; 65,536 tokens 65 and 49; 262,144 tokens 202 and 118.
+__global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbedArgs a, int log_groups) {
+  __shared__ int count[kMaxDealGroups];
+  const int groups = 1 << log_groups, n = static_cast<int>(a.N);
+  for (int g = threadIdx.x; g < groups; g += kSortThreads) count[g] = 0;
   __syncthreads();
-  int* const mine = hist + wave * a.bucket;
-  const int n = static_cast<int>(a.N), pad = static_cast<int>(a.padding);
-  const int chunk = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
-  const int begin = min(n, wave * chunk), end = min(n, begin + chunk);
-  const unsigned long long before = (1ull << lane) - 1ull;
-  int listed = 0, less = 0;
-  bool fits = true;
-  for (int base = begin; base < end; base += 256) {
-    int t[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int p = base + 64 * u + lane;
-      t[u] = p < end ? load_index(a.tokens, a.tokens64, p, a.V) : -1;
-      if (t[u] == pad) t[u] = -1;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool in = t[u] >= lo && t[u] < hi;
-      less += (t[u] >= 0 && t[u] < lo) ? 1 : 0;
-      const unsigned long long m = __ballot(in);
-      if (m == 0) continue;
-      const int k = __popcll(m);
-      fits = fits && listed + k <= kSortList;
-      if (in) {
-        atomicAdd(&mine[t[u] - lo], 1);
-        if (fits) {
-          const int at = listed + __popcll(m & before);
-          list_p[wave][at] = base + 64 * u + lane;
-          list_r[wave][at] = static_cast<uint16_t>(t[u] - lo);
-        }
-      }
-      listed += k;
-    }
+  const int begin = static_cast<int>(blockIdx.x) * a.chunk, end = min(n, begin + a.chunk);
+#pragma unroll 4
+  for (int p = begin + static_cast<int>(threadIdx.x); p < end; p += kSortThreads) {
+    const int64_t t = raw_token(a, p);
+    if (live_token(a, t)) atomicAdd(&count[static_cast<int>(t) & (groups - 1)], 1);
   }
-  less = static_cast<int>(wave_all_sum(static_cast<float>(less)));     // <= 2^24 per wave: exact
-  if (lane == 0) below[wave] = less;
   __syncthreads();
-  // per token: its total, the exclusive sum over the tokens of the bucket, then each wave's share behind the ones before it
-  int total = 0;
-  if (tid < own)
-    for (int w = 0; w < kSortWaves; ++w) total += hist[w * a.bucket + tid];
-  int run = total;
+  for (int g = threadIdx.x; g < groups; g += kSortThreads) a.counts[static_cast<int64_t>(blockIdx.x) * groups + g] = count[g];
+}
+
+// the lanes that agree with this one in the low `bits` bits of r, of those that are `in`: a ballot per bit, whatever r is
+__device__ __forceinline__ unsigned long long lanes_like(bool in, int r, int bits) {
+  unsigned long long same = __ballot(in);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (r >> b) & 1;
+    const unsigned long long m = __ballot(set);
+    same &= set ? m : ~m;
+  }
+  return same;
+}
+// Exclusive sum over the threads of a workgroup of kSortThreads (`sums`: one per wave); *all: the whole.
+__device__ __forceinline__ int scan_threads(int x, int* sums, int* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int run = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int got = __shfl(run, (lane - off) & 63, 64);
     if (lane >= off) run += got;
   }
   if (lane == 63) sums[wave] = run;
-  if (tid < own) totals[tid] = total;
   __syncthreads();
-  int start = run - total, all = 0;
+  int start = run - x, total = 0;
 #pragma unroll
   for (int w = 0; w < kSortWaves; ++w) {
-    start += below[w] + (w < wave ? sums[w] : 0);
-    all += below[w] + sums[w];
+    start += w < wave ? sums[w] : 0;
+    total += sums[w];
+  }
+  *all = total;
+  return start;
+}
+
+__global__ __launch_bounds__(kSortThreads) void embedding_deal_kernel(EmbedArgs a, int log_groups, int chunks) {
+  __shared__ int place[kSortWaves][kMaxDealGroups];
+  __shared__ int sums[kSortWaves];
+  const int groups = 1 << log_groups, n = static_cast<int>(a.N), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < kSortWaves * kMaxDealGroups; i += kSortThreads) place[0][i] = 0;
+  // where this chunk's share of each group begins (a thread per group: groups <= threads)
+  int before_me = 0, in_group = 0;
+  if (tid < groups) {
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+      const int k = a.counts[static_cast<int64_t>(c) * groups + tid];
+      in_group += k;
+      before_me += c < static_cast<int>(blockIdx.x) ? k : 0;
+    }
+  }
+  int all;
+  const int start = scan_threads(in_group, sums, &all);
+  if (blockIdx.x == 0) {
+    if (tid < groups) a.group_start[tid] = start;
+    if (tid == 0) a.group_start[groups] = all;
+  }
+  const int begin = static_cast<int>(blockIdx.x) * a.chunk + wave * (a.chunk / kSortWaves), end = min(n, begin + a.chunk / kSortWaves);
+  int* const mine = place[wave];
+  for (int p = begin + lane; p < end; p += 64) {
+    const int64_t t = raw_token(a, p);
+    if (live_token(a, t)) atomicAdd(&mine[static_cast<int>(t) & (groups - 1)], 1);
+  }
+  __syncthreads();
+  if (tid < groups) {
+    int at = start + before_me;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int k = place[w][tid];
+      place[w][tid] = at;
+      at += k;
+    }
+  }
+  __syncthreads();
+  const unsigned long long before = (1ull << lane) - 1ull;
+  for (int base = begin; base < end; base += 64) {
+    const int64_t t = base + lane < end ? raw_token(a, base + lane) : -1;
+    const bool in = live_token(a, t);
+    const int g = in ? static_cast<int>(t) & (groups - 1) : 0;
+    const unsigned long long same = lanes_like(in, g, log_groups);
+    const int at = in ? mine[g] : 0, rank = __popcll(same & before);
+    if (in) {
+      a.dealt_p[at + rank] = base + lane;
+      a.dealt_t[at + rank] = static_cast<int>(t);
+      if (rank == 0) mine[g] = at + __popcll(same);
+    }
+  }
+}
+
+template <typename TW, bool DEALT>
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs a, int log_groups) {
+  extern __shared__ int hist[];                     // [16][bucket] counts, then where the next one goes
+  __shared__ int list_p[kSortWaves][kSortList];
+  __shared__ uint16_t list_r[kSortWaves][kSortList];
+  __shared__ int sums[kSortWaves], below[kSortWaves], totals[kMaxBucket];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int group = static_cast<int>(blockIdx.x), groups = 1 << log_groups;
+  const int own = group < a.V ? (a.V - group + groups - 1) >> log_groups : 0;      // tokens of this workgroup
+  for (int i = tid; i < kSortWaves * a.bucket; i += kSortThreads) hist[i] = 0;
+  __syncthreads();
+  int* const mine = hist + wave * a.bucket;
+  const int first = DEALT ? a.group_start[group] : 0, n = DEALT ? a.group_start[group + 1] : static_cast<int>(a.N);
+  const int chunk = ((n - first + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
+  const int begin = min(n, first + wave * chunk), end = min(n, begin + chunk);
+  const unsigned long long before = (1ull << lane) - 1ull;
+  constexpr int kAhead = 8;
+  int64_t next[kAhead];
+  int next_p[DEALT ? kAhead : 1];
+  // f(which lanes hold a token of this workgroup, which one before it, the token's number here, the position), 64 positions at a time
+  auto scan = [&](auto f) {
+    auto fetch = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int p = base + 64 * u + lane;
+        if constexpr (DEALT) {
+          next[u] = p < end ? a.dealt_t[p] : -1;
+          next_p[u] = p < end ? a.dealt_p[p] : 0;
+        } else {
+          next[u] = p < end ? raw_token(a, p) : -1;
+        }
+      }
+    };
+    fetch(begin);
+    for (int base = begin; base < end; base += 64 * kAhead) {
+      int64_t now[kAhead];
+      int now_p[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        now[u] = next[u];
+        now_p[u] = DEALT ? next_p[DEALT ? u : 0] : base + 64 * u + lane;
+      }
+      if (base + 64 * kAhead < end) fetch(base + 64 * kAhead);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const bool live = DEALT ? now[u] >= 0 : live_token(a, now[u]);
+        const int t = static_cast<int>(now[u]), theirs = t & (groups - 1);
+        f(live && theirs == group, live && theirs < group, t >> log_groups, now_p[u]);
+      }
+    }
+  };
+  int listed = 0, less = 0;
+  bool fits = true;
+  scan([&](bool in, bool ahead, int r, int p) {
+    less += __popcll(__ballot(ahead));
+    const unsigned long long m = __ballot(in);
+    if (m == 0) return;
+    const int k = __popcll(m);
+    fits = fits && listed + k <= kSortList;
+    if (in) {
+      atomicAdd(&mine[r], 1);
+      if (fits) {
+        const int at = listed + __popcll(m & before);
+        list_p[wave][at] = p;
+        list_r[wave][at] = static_cast<uint16_t>(r);
+      }
+    }
+    listed += k;
+  });
+  if (lane == 0) below[wave] = less;
+  __syncthreads();
+  // per token: its total, the exclusive sum over the tokens of the workgroup, then each wave's share behind the ones before it
+  int total = 0;
+  if (tid < own)
+    for (int w = 0; w < kSortWaves; ++w) total += hist[w * a.bucket + tid];
+  if (tid < own) totals[tid] = total;
+  int all;
+  int start = first + scan_threads(total, sums, &all);
+  if constexpr (!DEALT) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      start += below[w];
+      all += below[w];
+    }
+  } else {
+    all += first;
   }
   if (tid < own) {
     for (int w = 0; w < kSortWaves; ++w) {
@@ -203,45 +346,53 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
       start += c;
     }
   }
-  if (tid == 0 && hi == a.V) a.header[0] = all;
+  if (tid == 0 && group == groups - 1) a.header[0] = all;
   __syncthreads();
-  // positions in order: lanes of one token take consecutive places (the lanes that agree with this one on every bit of the
-  // token's number in the bucket: a ballot per bit, whatever the tokens are)
+  // positions in order: lanes of one token take consecutive places
   const int bits = 32 - __builtin_clz(a.bucket | 1);
   auto place = [&](bool in, int r, int p) {
-    unsigned long long same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const bool set = (r >> b) & 1;
-      const unsigned long long m = __ballot(set);
-      same &= set ? m : ~m;
-    }
+    const unsigned long long same = lanes_like(in, r, bits);
     const int at = in ? mine[r] : 0, rank = __popcll(same & before);
     if (in) {
       a.order[at + rank] = p;
-      a.key[at + rank] = lo + r;
+      a.key[at + rank] = (r << log_groups) + group;
       if (rank == 0) mine[r] = at + __popcll(same);
     }
   };
-  if (fits) {
-    for (int base = 0; base < listed; base += 64) {
-      const bool in = base + lane < listed;
+  auto place_list = [&](int n_listed) {
+    for (int base = 0; base < n_listed; base += 64) {
+      const bool in = base + lane < n_listed;
       place(in, in ? list_r[wave][base + lane] : 0, in ? list_p[wave][base + lane] : 0);
     }
-  } else {
-    for (int base = begin; base < end; base += 64) {
-      const int p = base + lane;
-      int t = p < end ? load_index(a.tokens, a.tokens64, p, a.V) : -1;
-      if (t == pad) t = -1;
-      const bool in = t >= lo && t < hi;
-      place(in, in ? t - lo : 0, p);
-    }
+  };
+  if (!fits) {                    // the matches again, a list at a time
+    listed = 0;
+    scan([&](bool in, bool, int r, int p) {
+      const unsigned long long m = __ballot(in);
+      if (m == 0) return;
+      const int k = __popcll(m);
+      if (listed + k > kSortList) {
+        place_list(listed);
+        listed = 0;
+      }
+      if (in) {
+        const int at = listed + __popcll(m & before);
+        list_p[wave][at] = p;
+        list_r[wave][at] = static_cast<uint16_t>(r);
+      }
+      listed += k;
+    });
   }
+  place_list(listed);
   // rows of tokens that do not occur: zero
   const int64_t row_bytes = static_cast<int64_t>(a.D) * sizeof(TW);
   auto zero_row = [&](char* p, int64_t bytes) {
     if (bytes % 16 == 0) {
       const u32x4 z = {0u, 0u, 0u, 0u};
-      for (int64_t b = lane * 16; b < bytes; b += 1024) *reinterpret_cast<u32x4*>(p + b) = z;
+      if (a.stream_zeros)
+        for (int64_t b = lane * 16; b < bytes; b += 1024) __builtin_nontemporal_store(z, reinterpret_cast<u32x4*>(p + b));
+      else
+        for (int64_t b = lane * 16; b < bytes; b += 1024) *reinterpret_cast<u32x4*>(p + b) = z;
     } else if (bytes % 4 == 0) {
       for (int64_t b = lane * 4; b < bytes; b += 256) *reinterpret_cast<uint32_t*>(p + b) = 0u;
     } else {
@@ -250,8 +401,9 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
   };
   for (int r = wave; r < own; r += kSortWaves) {
     if (totals[r]) continue;
-    zero_row(static_cast<char*>(a.gw) + (lo + r) * row_bytes, row_bytes);
-    if (a.grho) zero_row(reinterpret_cast<char*>(a.grho) + (lo + r) * static_cast<int64_t>(a.D) * 4, static_cast<int64_t>(a.D) * 4);
+    const int64_t t = (static_cast<int64_t>(r) << log_groups) + group;
+    zero_row(static_cast<char*>(a.gw) + t * row_bytes, row_bytes);
+    if (a.grho) zero_row(reinterpret_cast<char*>(a.grho) + t * a.D * 4, static_cast<int64_t>(a.D) * 4);
   }
 }
 
@@ -342,11 +494,12 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(EmbedArgs a, int 
   }
 }
 
-// One workgroup per (piece, 64 * VEC columns): if a run begins in this piece and goes on behind it, add its parts.  The four
-// waves take every fourth part; their sums are added in order.
+constexpr int kJoinBlock = 512;
+// One workgroup per (piece, 64 * VEC columns): if a run begins in this piece and goes on behind it, add its parts.  The
+// eight waves take every eighth part; their sums are added in order.
 template <typename TW, int NOISE, int VEC>
-__global__ __launch_bounds__(kBlock) void embedding_join_kernel(EmbedArgs a, int column_tiles) {
-  constexpr int NACC = NOISE == kNoisePosition ? 2 : 1, kWaves = kBlock / 64;
+__global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(EmbedArgs a, int column_tiles) {
+  constexpr int NACC = NOISE == kNoisePosition ? 2 : 1, kWaves = kJoinBlock / 64;
   __shared__ float sums[kWaves - 1][NACC][64 * VEC];
   const int piece = static_cast<int>(blockIdx.x) / column_tiles;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -354,7 +507,7 @@ __global__ __launch_bounds__(kBlock) void embedding_join_kernel(EmbedArgs a, int
   const int n = a.header[0], s0 = piece * a.piece, s1 = s0 + a.piece;
   if (s1 >= n) return;
   const int key = a.key[s1 - 1];
-  if (a.key[s1] != key || (s0 > 0 && a.key[s0 - 1] == key)) return;     // (keys are sorted: equal ends mean equal in between)
+  if (a.key[s1] != key || (s0 > 0 && a.key[s0 - 1] == key)) return;     // (a token's positions are side by side: equal ends mean equal in between)
   // parts of the pieces behind: those whose first key is this one
   int behind = 0;
   for (;;) {
@@ -401,29 +554,58 @@ __global__ __launch_bounds__(kBlock) void embedding_join_kernel(EmbedArgs a, int
   embedding_finish<TW, NOISE, VEC>(a, key, d, acc, acc2);
 }
 
-// positions per piece: short pieces keep enough waves in flight when there are few tokens, long ones write fewer parts
-static int embedding_piece(int64_t n) { return n <= 8192 ? 16 : n <= 65536 ? 32 : 64; }
+constexpr int64_t kDealTokens = 49152;
+// positions per workgroup of the dealing kernels (0: no dealing): at most 256 chunks, whole waves of 64 positions
+static int embedding_chunk(int64_t n) {
+  if (n < kDealTokens) return 0;
+  const int64_t chunk = std::max<int64_t>(4096, (n + 255) / 256);
+  return static_cast<int>((chunk + 1023) / 1024 * 1024);
+}
+// When the table's gradient and what is read beside it are well beyond the 256 MB memory-side cache, zero rows that stay in it are
+// pushed out again by the rows that the sums read: 65,536 tokens, 131,072 x 1,024 bf16, 131 us against 105 us past the caches (512
+// tokens: 54 against 62; 92 MB of zero rows: 28 against 30).
+constexpr int64_t kStreamZeros = 320 << 20;
+
+// positions per piece: short pieces keep enough waves in flight when there are few tokens (4,800 x 768 Gaussian: sums 13.9 us with
+// 8, 17.7 with 16, 51 with 64), long ones leave fewer parts to join (1,048,576 tokens: 41 us with 64, 138 with 16)
+static int embedding_piece(int64_t n) { return n <= 8192 ? 8 : n <= 32768 ? 16 : n <= 65536 ? 32 : 64; }
+
+constexpr int64_t kFwdManyRows = 16384;
 
 template <typename TW, typename TO, int NOISE, int VEC>
 static int embedding_fwd_launch(const EmbedArgs& a, hipStream_t s) {
   const int vecs = (a.D + VEC - 1) / VEC;
   int log_lanes = 3;
   while (log_lanes < 6 && (1 << log_lanes) < vecs) ++log_lanes;
-  const int64_t blocks = ((a.N << log_lanes) + kBlock - 1) / kBlock;
-  hipLaunchKernelGGL((embedding_fwd_kernel<TW, TO, NOISE, VEC>), dim3(static_cast<unsigned>(blocks)), dim3(kBlock), 0, s, a, log_lanes);
-  return to_err(hipGetLastError());
+  auto go = [&](auto kernel, int rows) {
+    const int64_t blocks = ((((a.N + rows - 1) / rows) << log_lanes) + kBlock - 1) / kBlock;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kBlock), 0, s, a, log_lanes);
+    return to_err(hipGetLastError());
+  };
+  if (a.N >= kFwdManyRows) return go(&embedding_fwd_kernel<TW, TO, NOISE, VEC, 4>, 4);
+  return go(&embedding_fwd_kernel<TW, TO, NOISE, VEC, 1>, 1);
 }
 template <typename TW, typename TG, int NOISE, int VEC>
 static int embedding_bwd_launch(const EmbedArgs& a, hipStream_t s) {
-  const int buckets = (a.V + a.bucket - 1) / a.bucket;
-  hipLaunchKernelGGL((embedding_sort_kernel<TW>), dim3(buckets), dim3(kSortThreads), sizeof(int) * kSortWaves * a.bucket, s, a);
+  const dim3 groups(1u << a.log_groups);
+  const size_t lds = sizeof(int) * kSortWaves * a.bucket;
+  if (a.chunk > 0) {
+    const int chunks = static_cast<int>((a.N + a.chunk - 1) / a.chunk);
+    hipLaunchKernelGGL(embedding_count_kernel, dim3(chunks), dim3(kSortThreads), 0, s, a, a.log_groups);
+    if (const int rc = to_err(hipGetLastError())) return rc;
+    hipLaunchKernelGGL(embedding_deal_kernel, dim3(chunks), dim3(kSortThreads), 0, s, a, a.log_groups, chunks);
+    if (const int rc = to_err(hipGetLastError())) return rc;
+    hipLaunchKernelGGL((embedding_sort_kernel<TW, true>), groups, dim3(kSortThreads), lds, s, a, a.log_groups);
+  } else {
+    hipLaunchKernelGGL((embedding_sort_kernel<TW, false>), groups, dim3(kSortThreads), lds, s, a, a.log_groups);
+  }
   if (const int rc = to_err(hipGetLastError())) return rc;
   if (a.N == 0) return 0;
   const int tiles = (a.D + 64 * VEC - 1) / (64 * VEC), pieces = static_cast<int>((a.N + a.piece - 1) / a.piece);
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(pieces) * tiles + kBlock / 64 - 1) / (kBlock / 64));
   hipLaunchKernelGGL((embedding_sum_kernel<TW, TG, NOISE, VEC>), dim3(blocks), dim3(kBlock), 0, s, a, tiles);
   if (const int rc = to_err(hipGetLastError())) return rc;
-  if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<TW, NOISE, VEC>), dim3(pieces * tiles), dim3(kBlock), 0, s, a, tiles);
+  if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<TW, NOISE, VEC>), dim3(pieces * tiles), dim3(kJoinBlock), 0, s, a, tiles);
   return to_err(hipGetLastError());
 }
 
@@ -484,9 +666,12 @@ extern "C" int bde_embedding_fwd(const void* weight, int weight_dtype, int64_t l
   return embedding_dispatch<false>(a, weight_dtype, out_dtype, noise, static_cast<hipStream_t>(stream));
 }
 
+constexpr int64_t kDealBytes = 4 * (256 * kMaxDealGroups + kMaxDealGroups + 64);      // counts and group starts
+
 extern "C" size_t bde_embedding_bwd_ws_bytes(int64_t N, int64_t D, int noise) {
   if (N < 0 || N > BDE_EMBEDDING_MAX_TOKENS || D < 1 || D > BDE_EMBEDDING_MAX_DIM) return 0;
-  const int64_t lists = 256 + 2 * ((4 * N + 255) / 256 * 256);
+  const int64_t list = (4 * N + 255) / 256 * 256;
+  const int64_t lists = 256 + 2 * list + (embedding_chunk(N) > 0 ? 2 * list + kDealBytes : 0);
   const int64_t pieces = (N + embedding_piece(N) - 1) / embedding_piece(N);
   return static_cast<size_t>(lists + pieces * 2 * (noise == kNoisePosition ? 2 : 1) * D * 4 + 16);
 }
@@ -509,15 +694,28 @@ extern "C" int bde_embedding_bwd(const void* g, int g_dtype, int64_t ldg, const 
   a.header = reinterpret_cast<int*>(base);
   a.order = reinterpret_cast<int*>(base + 256);
   a.key = reinterpret_cast<int*>(base + 256 + list);
-  a.part = reinterpret_cast<float*>(base + 256 + 2 * list);
+  // 256 workgroups (one per CU), or as many as keep a workgroup's counts in LDS; no more than tokens
+  a.log_groups = 8;
+  while ((V + (1 << a.log_groups) - 1) >> a.log_groups > kMaxBucket) ++a.log_groups;
+  while (a.log_groups > 0 && (int64_t{1} << (a.log_groups - 1)) >= V) --a.log_groups;
+  a.bucket = static_cast<int>((V + (1 << a.log_groups) - 1) >> a.log_groups);
+  char* rest = base + 256 + 2 * list;
+  if (embedding_chunk(N) > 0) {
+    if ((1 << a.log_groups) <= kMaxDealGroups) a.chunk = embedding_chunk(N);
+    a.counts = reinterpret_cast<int*>(rest);
+    a.group_start = a.counts + 256 * kMaxDealGroups;
+    a.dealt_p = reinterpret_cast<int*>(rest + kDealBytes);
+    a.dealt_t = reinterpret_cast<int*>(rest + kDealBytes + list);
+    rest += kDealBytes + 2 * list;
+  }
+  a.part = reinterpret_cast<float*>(rest);
   a.piece = embedding_piece(N);
-  // 256 workgroups (one per CU), or as many as keep a bucket's counts in LDS
-  const int64_t want = std::max<int64_t>(kCUs, (V + kMaxBucket - 1) / kMaxBucket);
-  a.bucket = static_cast<int>((V + want - 1) / want);
+  a.stream_zeros = V * D * static_cast<int64_t>(dtype_bytes(weight_dtype) + (g_rho ? 4 : 0)) +
+                       N * D * static_cast<int64_t>(dtype_bytes(g_dtype) + (noise == kNoisePosition && eps ? 4 : 0)) > kStreamZeros;
   return embedding_dispatch<true>(a, weight_dtype, g_dtype, noise, static_cast<hipStream_t>(stream));
 }
 
 extern "C" __attribute__((visibility("hidden"))) int bde_internal_load_embedding(void) {
   hipFuncAttributes attr;
-  return to_err(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&embedding_sort_kernel<float>)));
+  return to_err(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&embedding_sort_kernel<float, false>)));
 }

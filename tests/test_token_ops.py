@@ -158,6 +158,24 @@ def test_embedding_many_positions_of_few_tokens(backend):
     check_embedding(backend, tokens, torch.randn(3, 4, generator=g), None, scale=0.5)
 
 
+def test_embedding_of_many_rows(backend):
+    """Enough rows for four to a group of lanes, and a last group that is not full."""
+    g = gen(6)
+    tokens = torch.randint(0, 9, (16387,), generator=g)
+    check_embedding(backend, tokens, torch.randn(9, 8, generator=g).bfloat16(), None, scale=2.0, pad=4)
+    mean, rho = torch.randn(9, 3, generator=g), torch.randn(9, 3, generator=g) - 2
+    check_embedding(backend, tokens, mean, rho, noise="position", eps=torch.randn(16387, 3, generator=g))
+
+
+@pytest.mark.parametrize("v", [5, 1500])
+def test_embedding_gradient_of_many_tokens(backend, v):
+    """Enough tokens to be dealt out to the sort's workgroups first: one frequent token, padding, tokens outside the table."""
+    g = gen(v)
+    tokens = torch.where(torch.rand(49200, generator=g) < 0.3, 3, torch.randint(-1, v + 1, (49200,), generator=g))
+    check_embedding(backend, tokens, torch.randn(v, 4, generator=g), None, pad=1)
+    check_embedding(backend, tokens.int(), torch.randn(v, 2, generator=g), None)
+
+
 def test_embedding_strided_operands(backend):
     """Rows that lie apart, rows off a 16-byte border, a transposed table, a broadcast and a strided gradient."""
     g = gen(11)

@@ -112,6 +112,8 @@ ROWS = {
     "embedding_fwd_kernel": ("the lookup, scaling and noise of a token model's first layer (torch's index_select + mul + add)", "rows touched + `N·D` out", "see §5.3", TOK,
                              "`test_embedding_*`, `test_gaussian_embedding`"),
     "embedding_sort_kernel": ("positions sorted by token in one launch; zero rows of absent tokens", "`8·N` B + the absent rows", "see §5.3", TOK, "same"),
+    "embedding_count_kernel": ("many tokens: how many of each chunk go to each workgroup of the sort", "`8·N` B", "see §5.3", TOK, "`test_embedding_gradient_of_many_tokens`"),
+    "embedding_deal_kernel": ("many tokens: positions dealt out to the sort's workgroups, in order", "`16·N` B", "see §5.3", TOK, "same test"),
     "embedding_sum_kernel": ("the tokens' gradient rows, added in order (torch: atomics)", "`N·D` in, touched rows out", "see §5.3", TOK, "same"),
     "embedding_join_kernel": ("runs that cross a piece of the sorted list", "latency", "see §5.3", TOK, "`test_embedding_token_patterns`"),
     "topk_logits_kernel": ("a teacher's k largest logits, their classes and the log-sum of the rest", "`N·V` read once", "see §5.3", TOK, "`test_topk_*`"),
