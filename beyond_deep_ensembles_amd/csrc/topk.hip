@@ -56,12 +56,40 @@ __device__ __forceinline__ int row_count(int n, int* slots) {
   return r;
 }
 
+// One wave: a key that at least k of the 64 * M keys reach (k <= 64 * M) and, unless they are equal, not many more -- bisection over
+// the keys, counts by ballot.
+template <int M>
+__device__ __forceinline__ uint32_t reach_of(const uint32_t* keys, int k) {
+  uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    low = min(low, keys[i]);
+    high = max(high, keys[i]);
+  }
+  // ends of the range over the wave: the upper 16 bits are exact as floats
+  uint32_t lo = static_cast<uint32_t>(-wave_all_max(-static_cast<float>(low >> 16))) << 16;
+  uint32_t hi = (static_cast<uint32_t>(wave_all_max(static_cast<float>(high >> 16))) << 16) | 0xFFFFu;
+  while (lo < hi) {            // invariant: count(>= lo) >= k, count(> hi) < k
+    const uint32_t mid = lo + ((hi - lo) >> 1) + 1u;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) n += __popcll(__ballot(keys[i] >= mid));
+    if (n >= k) {
+      lo = mid;
+      if (n <= k + (k >> 2) + 4) break;
+    } else {
+      hi = mid - 1u;
+    }
+  }
+  return lo;
+}
+
 // NT threads per row: its first NT * NV granules of 16 bytes are kept in registers, what a longer row has
 // beyond them is read again (from the caches) by the second pass.
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(TopkArgs a) {
   constexpr int GN = Granule<T>::N, W = NT / 64, ROWS = kRowsPerGroup<NT>;
-  constexpr int kCap = NT == 64 ? 128 : 1024;        // entries of the candidate list
+  constexpr int kCap = NT == 64 ? 64 + 64 * NV : 1024;      // entries of the candidate list
   const int row_of_group = ROWS > 1 ? __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / NT) : 0;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + row_of_group;
   if (ROWS > 1 && row >= a.N) return;                // (waves that share a workgroup share nothing else)
@@ -70,7 +98,7 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
   const RowView<T> z(static_cast<const T*>(a.z) + row * a.ldz, a.V);
   __shared__ uint64_t cand_[ROWS][kCap];
   __shared__ int hits_[ROWS][kCap];
-  __shared__ uint32_t maxima_[ROWS][NT];
+  __shared__ uint32_t maxima_[ROWS][W > 1 ? NT : 1];
   __shared__ float slots_[ROWS][2 * W];
   __shared__ int counts_[ROWS][W];
   __shared__ uint32_t bound_[ROWS];
@@ -96,43 +124,43 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
     }
     for (int g = tid + NV * NT; g < z.granules; g += NT) f(z.load(g), g);
   };
+  // the maxima the bound comes from: each thread's, or -- a row of one wave, when k comes near its 64 lanes -- each granule's
   float best = neg_inf();
-  each([&](const u32x4& x, int) {
+  uint32_t own[NV];
+  const bool by_granule = W == 1 && a.K > 24;
+  if (by_granule) {
 #pragma unroll
-    for (int i = 0; i < GN; ++i) best = fmaxf(best, granule_get<T>(x, i));
-  });
-  maxima[tid] = order_key(best);
+    for (int j = 0; j < NV; ++j) {
+      float g = neg_inf();
+      if (j * NT < z.granules) {
+#pragma unroll
+        for (int i = 0; i < GN; ++i) g = fmaxf(g, granule_get<T>(reg[j], i));
+      }
+      own[j] = order_key(g);
+    }
+  } else {
+    each([&](const u32x4& x, int) {
+#pragma unroll
+      for (int i = 0; i < GN; ++i) best = fmaxf(best, granule_get<T>(x, i));
+    });
+  }
+  if constexpr (W > 1) maxima[tid] = order_key(best);
   if (tid == 0) n_hit = n_cand = 0;
   row_sync<NT>();
-  // wave 0: a bound that at least k of the NT maxima reach and not many more (bisection over the keys, counts by ballot)
   if (tid < 64) {
-    uint32_t lo = kKeyNegInf;
-    if (a.K < NT) {
-      uint32_t m[W];
-      uint32_t low = 0xFFFFFFFFu, high = 0;
+    uint32_t lo = 0;
+    if constexpr (W > 1) {
+      uint32_t top[W];
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        m[i] = maxima[lane + 64 * i];
-        low = min(low, m[i]);
-        high = max(high, m[i]);
-      }
-      // ends of the range over the wave: the upper 16 bits are exact as floats
-      lo = max(lo, static_cast<uint32_t>(-wave_all_max(-static_cast<float>(low >> 16))) << 16);
-      uint32_t hi = (static_cast<uint32_t>(wave_all_max(static_cast<float>(high >> 16))) << 16) | 0xFFFFu;
-      while (lo < hi) {          // invariant: count(>= lo) >= k, count(> hi) < k
-        const uint32_t mid = lo + ((hi - lo) >> 1) + 1u;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < W; ++i) n += __popcll(__ballot(m[i] >= mid));
-        if (n >= a.K) {
-          lo = mid;
-          if (n <= a.K + (a.K >> 2) + 4) break;
-        } else {
-          hi = mid - 1u;
-        }
-      }
+      for (int i = 0; i < W; ++i) top[i] = maxima[lane + 64 * i];
+      if (a.K < NT) lo = reach_of<W>(top, a.K);
+    } else if (by_granule) {
+      if (a.K < NT * NV) lo = reach_of<NV>(own, a.K);
+    } else {
+      const uint32_t top = order_key(best);
+      lo = reach_of<1>(&top, a.K);
     }
-    if (lane == 0) bound = lo;
+    if (lane == 0) bound = max(lo, kKeyNegInf);
   }
   row_sync<NT>();
   const float c = a.inv_tau * kLog2e;
@@ -258,20 +286,20 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
   row_sync<NT>();
   // the candidates left over, relative to the largest of them
   const int left = n - a.K;
-  float more = 0.0f, top = 0.0f;
+  float more = 0.0f, from = 0.0f;
   if (left > 0) {                              // (only without the bisection: then a.K + left candidates were listed)
     const float first = order_value(static_cast<uint32_t>(cand[0] >> 32));
-    top = first - first == 0.0f ? first : 0.0f;
+    from = first - first == 0.0f ? first : 0.0f;
     for (int i = tid; i < left; i += NT) {
       const uint32_t key = static_cast<uint32_t>(cand[i] >> 32);
-      more += exp2_hw(((key == 0xFFFFFFFFu ? __builtin_nanf("") : order_value(key)) - top) * c);
+      more += exp2_hw(((key == 0xFFFFFFFFu ? __builtin_nanf("") : order_value(key)) - from) * c);
     }
   }
   more = row_all_sum<NT>(more, slots + W);
   if (tid == 0) {
     float r = neg_inf();
-    if (left > 0 && more != 0.0f)              // ref <= top: the others' sum relative to top
-      r = top * a.inv_tau + kLn2 * __builtin_amdgcn_logf(more + others * exp2_hw((ref - top) * c));
+    if (left > 0 && more != 0.0f)              // ref <= from: the others' sum relative to it
+      r = from * a.inv_tau + kLn2 * __builtin_amdgcn_logf(more + others * exp2_hw((ref - from) * c));
     else if (others != 0.0f)
       r = ref * a.inv_tau + kLn2 * __builtin_amdgcn_logf(others);
     a.rest[row] = r;
@@ -285,22 +313,22 @@ static int topk_launch(const TopkArgs& a, hipStream_t s) {
   return to_err(hipGetLastError());
 }
 // Threads and registers by the granules of a row, as distill.hip: as few waves as hold the row, four to eight granules a thread.
-// The bound comes from the threads' maxima, so a row gets several times k threads.
+// The bound comes from the threads' (one wave: the granules') maxima, so a row has at least about twice k of them.
 // bf16, k = 64: 32,000 classes 36 us with 512 x 8 for 2,048 rows (47 with 1024 x 4); 131,072 classes 280 us with 1024 x 8 and the
-// row's other half read again, 330 us with 1024 x 16 (one workgroup per CU, whose phases then overlap with no other's).
+// row's other half read again, 330 us with 1024 x 16 (one workgroup per CU, whose phases then overlap with no other's); one row
+// of them 16 us with 1024 x 16, 19 with 1024 x 8.
 template <typename T>
 static int topk_pick(const TopkArgs& a, hipStream_t s) {
   constexpr int GN = Granule<T>::N;
   const bool aligned = aligned16(a.z) && (a.ldz % GN == 0 || a.N == 1);
   const int granules = (a.V + (aligned ? 0 : GN - 1) + GN - 1) / GN;
-  if (a.K <= 24) {
-    if (granules <= 64) return topk_launch<T, 64, 1>(a, s);
-    if (granules <= 256) return topk_launch<T, 64, 4>(a, s);
-  }
+  if (granules <= 64 && 2 * a.K <= granules + 16) return topk_launch<T, 64, 1>(a, s);
+  if (granules <= 256 && 2 * a.K <= granules + 16) return topk_launch<T, 64, 4>(a, s);
   if (granules <= 1024) return topk_launch<T, 256, 4>(a, s);
   if (granules <= 2048) return topk_launch<T, 256, 8>(a, s);
   if (granules <= 4096) return topk_launch<T, 512, 8>(a, s);
   if (granules <= 6144) return topk_launch<T, 512, 12>(a, s);
+  if (a.N <= kCUs && granules <= 16384) return topk_launch<T, 1024, 16>(a, s);
   return topk_launch<T, 1024, 8>(a, s);
 }
 

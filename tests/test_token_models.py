@@ -10,7 +10,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 import beyond_deep_ensembles_amd as bde
-from tests.test_token_ops import BF16, F32, U, backend, distill64, gen, teacher  # noqa: F401  (backend: the fixture)
+from tests.test_token_ops import BF16, F32, U, backend, distill64, exponent_error, gen, teacher  # noqa: F401  (backend: the fixture)
 
 
 def test_scaled_embedding_is_an_embedding(backend):
@@ -275,7 +275,9 @@ def test_offsets_beyond_32_bits():
     z[-2:] = last
     top = bde.topk_logits(z, 8)
     small = bde.topk_logits(last, 8)
-    assert torch.equal(top.indices[-2:], small.indices) and torch.equal(top.rest[-2:], small.rest)
+    assert torch.equal(top.indices[-2:], small.indices) and torch.equal(top.values[-2:], small.values)
+    # (two rows are worked on in pieces, many are not: other orders of the same sum, each within exponent_error of it; |z| < 15)
+    assert (top.rest[-2:] - small.rest).abs().max().item() <= 2 * exponent_error(45.0, v)
     weight = torch.zeros(n, device=dev)
     weight[-2:] = 1.0
     x = z.requires_grad_()
