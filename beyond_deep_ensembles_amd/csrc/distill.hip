@@ -33,6 +33,7 @@ struct DistillArgs {
   void* grad;                // [N, ldg]
   int64_t ldg;
   int N, V, K;
+  int64_t row0;              // first row of this launch
   int stream_out;            // the gradient is too large to stay in the caches until it is read
   float coef;                // factor of every row's loss
   float inv_tau;
@@ -47,7 +48,7 @@ template <typename T, int NT, int NV, bool GRAD>
 __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(DistillArgs a) {
   constexpr int GN = Granule<T>::N, W = NT / 64, ROWS = kRowsPerGroup<NT>;
   const int mine = ROWS > 1 ? __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / NT) : 0;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + mine;
+  const int64_t row = a.row0 + static_cast<int64_t>(blockIdx.x) * ROWS + mine;
   if (ROWS > 1 && row >= a.N) return;          // (waves that share a workgroup share nothing else)
   const int tid = static_cast<int>(threadIdx.x) % NT, lane = tid & 63, wave = tid >> 6;
   const int wave_first = __builtin_amdgcn_readfirstlane(tid);       // a wave whose granules all lie behind the row skips them
@@ -345,11 +346,15 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* loss, in
 constexpr int64_t kStreamBytes = 64 << 20;
 
 template <typename T, int NT, int NV, bool GRAD>
-static int distill_launch(const DistillArgs& a, hipStream_t s) {
+static int distill_launch(DistillArgs a, hipStream_t s) {
   constexpr int ROWS = kRowsPerGroup<NT>;
   const size_t lds = 4 * ROWS * (static_cast<size_t>((a.V + Granule<T>::N + 31) / 32 + 1) + 3 * static_cast<size_t>(a.K));
-  hipLaunchKernelGGL((distill_topk_kernel<T, NT, NV, GRAD>), dim3((a.N + ROWS - 1) / ROWS), dim3(NT * ROWS), lds, s, a);
-  return to_err(hipGetLastError());
+  for (a.row0 = 0; a.row0 < a.N; a.row0 += kRowsPerLaunch) {
+    const int rows = static_cast<int>(std::min<int64_t>(kRowsPerLaunch, a.N - a.row0));
+    hipLaunchKernelGGL((distill_topk_kernel<T, NT, NV, GRAD>), dim3((rows + ROWS - 1) / ROWS), dim3(NT * ROWS), lds, s, a);
+    if (const int rc = to_err(hipGetLastError())) return rc;
+  }
+  return 0;
 }
 // Threads and registers by the granules of a row: four to eight granules a thread (enough loads in flight, several rows per CU
 // whose phases overlap) and as few waves as hold the row -- a barrier costs per wave.  bf16, forward with gradient: 32,000 classes

@@ -404,8 +404,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_logits(const at::Tensor& log
   const int64_t n = z.size(0), v = z.size(1);
   int max_v = 0, max_k = 0;
   bde_topk_limits(&max_v, &max_k);
-  if (k < 1 || k > v || k > max_k || v > max_v)
-    refuse("topk_logits: 1 <= k <= min(V, ", max_k, ") and V <= ", max_v, " supported, got k=", k, ", V=", v);
+  if (k < 1 || k > v || k > max_k || v > max_v || n > INT32_MAX)
+    refuse("topk_logits: 1 <= k <= min(V, ", max_k, "), V <= ", max_v, " and fewer than 2^31 rows supported, got k=", k, ", V=", v, ", ", n, " rows");
   c10::DeviceGuard guard(z.device());
   std::vector<int64_t> shape = logits.sizes().vec();
   shape.back() = k;
@@ -494,7 +494,7 @@ at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& values,
   int max_v = 0, max_k = 0;
   bde_distill_limits(&max_v, &max_k);
   if (k < 1 || k > max_k || v > max_v || n > INT32_MAX)
-    refuse("distillation_loss: 1 <= K <= ", max_k, " and 1 <= V <= ", max_v, " supported, got K=", k, ", V=", v);
+    refuse("distillation_loss: 1 <= K <= ", max_k, ", 1 <= V <= ", max_v, " and fewer than 2^31 rows supported, got K=", k, ", V=", v, ", ", n, " rows");
   if (type_code(values.scalar_type()) < 0) refuse("values: expected float32 / bfloat16 / float16, got ", values.scalar_type());
   need_index_type(indices, "indices");
   same_device(logits, values, "values");

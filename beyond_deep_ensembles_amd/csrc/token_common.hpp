@@ -127,6 +127,7 @@ __device__ __forceinline__ float wave_all_max(float x) {
 // only the wait for the LDS operations.
 template <int NT>
 constexpr int kRowsPerGroup = NT == 64 ? 4 : 1;
+constexpr int64_t kRowsPerLaunch = 1 << 21;      // (a launch holds fewer than 2^32 threads)
 template <int NT>
 __device__ __forceinline__ void row_sync() {
   if constexpr (NT == 64) {

@@ -21,6 +21,7 @@ struct TopkArgs {
   float* rest;        // [N] or NULL
   int N, V, K;
   float inv_tau;
+  int64_t row0;       // first row of this launch
 };
 
 constexpr int kTopkMaxK = 256;
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
   constexpr int GN = Granule<T>::N, W = NT / 64, ROWS = kRowsPerGroup<NT>;
   constexpr int kCap = NT == 64 ? 64 + 64 * NV : 1024;      // entries of the candidate list
   const int row_of_group = ROWS > 1 ? __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / NT) : 0;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + row_of_group;
+  const int64_t row = a.row0 + static_cast<int64_t>(blockIdx.x) * ROWS + row_of_group;
   if (ROWS > 1 && row >= a.N) return;                // (waves that share a workgroup share nothing else)
   const int tid = static_cast<int>(threadIdx.x) % NT, lane = tid & 63;
   const int wave_first = __builtin_amdgcn_readfirstlane(tid);       // a wave whose granules all lie behind the row skips them
@@ -307,10 +308,14 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
 }
 
 template <typename T, int NT, int NV>
-static int topk_launch(const TopkArgs& a, hipStream_t s) {
+static int topk_launch(TopkArgs a, hipStream_t s) {
   constexpr int ROWS = kRowsPerGroup<NT>;
-  hipLaunchKernelGGL((topk_logits_kernel<T, NT, NV>), dim3((a.N + ROWS - 1) / ROWS), dim3(NT * ROWS), 0, s, a);
-  return to_err(hipGetLastError());
+  for (a.row0 = 0; a.row0 < a.N; a.row0 += kRowsPerLaunch) {
+    const int rows = static_cast<int>(std::min<int64_t>(kRowsPerLaunch, a.N - a.row0));
+    hipLaunchKernelGGL((topk_logits_kernel<T, NT, NV>), dim3((rows + ROWS - 1) / ROWS), dim3(NT * ROWS), 0, s, a);
+    if (const int rc = to_err(hipGetLastError())) return rc;
+  }
+  return 0;
 }
 // Threads and registers by the granules of a row, as distill.hip: as few waves as hold the row, four to eight granules a thread.
 // The bound comes from the threads' (one wave: the granules') maxima, so a row has at least about twice k of them.
@@ -349,7 +354,7 @@ extern "C" int bde_topk_logits(const void* logits, int dtype, int64_t ldz, float
     return BDE_ERR_INVALID;
   if (N == 0) return 0;
   if (!logits || !values || !indices || reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dtype) != 0) return BDE_ERR_INVALID;
-  const TopkArgs a{logits, ldz, values, indices, rest, N, V, K, 1.0f / temperature};
+  const TopkArgs a{logits, ldz, values, indices, rest, N, V, K, 1.0f / temperature, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == BDE_F32) return topk_pick<float>(a, s);
   if (dtype == BDE_BF16) return topk_pick<bf16_t>(a, s);

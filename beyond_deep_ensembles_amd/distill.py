@@ -54,8 +54,8 @@ def topk_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, _ops=
         return TopLogits(*native.topk_logits(logits, k, temperature))
     rows = _logit_rows(logits.detach())
     n, v = rows.shape
-    if not 1 <= k <= min(v, 256) or v > 262144:
-        raise BdeKernelError(f"topk_logits: 1 <= k <= min(V, 256) and V <= 262144 supported, got k={k}, V={v}")
+    if not 1 <= k <= min(v, 256) or v > 262144 or n >= 2 ** 31:
+        raise BdeKernelError(f"topk_logits: 1 <= k <= min(V, 256), V <= 262144 and fewer than 2^31 rows supported, got k={k}, V={v}, {n} rows")
     shape = logits.shape[:-1]
     values = torch.empty((n, k), dtype=rows.dtype, device=rows.device)
     indices = torch.empty((n, k), dtype=torch.int64, device=rows.device)
@@ -133,8 +133,9 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
         raise BdeKernelError(f"distillation_loss: values and indices of shape {lead + ('K',)} expected, got {tuple(values.shape)} and "
                              f"{tuple(indices.shape)}")
     k = values.shape[-1]
-    if not 1 <= k <= 1024 or not 1 <= v <= 262144:
-        raise BdeKernelError(f"distillation_loss: 1 <= K <= 1024 and 1 <= V <= 262144 supported, got K={k}, V={v}")
+    if not 1 <= k <= 1024 or not 1 <= v <= 262144 or n >= 2 ** 31:
+        raise BdeKernelError(f"distillation_loss: 1 <= K <= 1024, 1 <= V <= 262144 and fewer than 2^31 rows supported, got K={k}, V={v}, "
+                             f"{n} rows")
     for name, t in (("rest", rest), ("weight", weight)):
         if t is not None and tuple(t.shape) != lead:
             raise BdeKernelError(f"{name}: expected shape {lead}, got {tuple(t.shape)}")

@@ -44,7 +44,7 @@ extern "C" {
 #define BDE_F32 0
 #define BDE_BF16 1
 #define BDE_F16 2
-#define BDE_EMBEDDING_MAX_TOKENS (1 << 28)
+#define BDE_EMBEDDING_MAX_TOKENS (1 << 25)
 #define BDE_EMBEDDING_MAX_ROWS (1 << 24)
 #define BDE_EMBEDDING_MAX_DIM 16384
 

@@ -161,6 +161,24 @@ def test_a_student_distilled_from_an_ensemble(backend):
         assert torch.allclose(got.cpu().double(), ref, rtol=0, atol=1e-5 * float(ref.abs().max()))
 
 
+def test_a_bbb_step_over_an_embedding_and_a_linear_layer(backend):
+    """BBBOptimizer drives the mean-field embedding as it does the other layers: its mean and rho are paired, the KL is fused, a
+    step moves both, and the padding row's mean moves by the prior alone."""
+    ops, dev = backend
+    torch.manual_seed(3)
+    prior = bde.GaussianPrior(0, 1.0)
+    net = nn.ModuleDict(dict(emb=bde.BBBEmbedding(12, 8, prior, padding_idx=0, rng="philox", _ops=ops), head=bde.BBBLinear(8, 5, prior, prior, _ops=ops))).to(dev)
+    z, values, indices, rest = teacher(6, 5, 2, F32, 1)
+    top = [t.to(dev) for t in (values, indices, rest)]
+    tokens = torch.randint(0, 12, (6, 4), generator=gen(2)).to(dev)
+    opt = bde.BBBOptimizer(list(net.parameters()), torch.optim.SGD(net.parameters(), lr=0.1), prior, dataset_size=6, mc_samples=2, _ops=ops)
+    before = {k: v.detach().clone() for k, v in net.named_parameters()}
+    loss = opt.step(lambda: bde.distillation_loss(net["head"](net["emb"](tokens).mean(1)), *top, _ops=ops), lambda l: l.backward())
+    assert math.isfinite(float(loss))
+    for k, v in net.named_parameters():
+        assert torch.isfinite(v).all() and not torch.equal(v, before[k]), k
+
+
 # ---------------------------------------------------------------- device --
 def _hip():
     from beyond_deep_ensembles_amd.ops import HipOps
@@ -233,20 +251,18 @@ def test_a_backward_captured_without_its_forward():
     """The graph then computes the gradient itself, from the logits as they are at each replay."""
     ops, dev = _hip(), "cuda:0"
     z, values, indices, rest = (t.to(dev) for t in teacher(20, 2000, 8, F32, 0))
-    x = z.clone().requires_grad_()
+    (want,) = torch.autograd.grad(bde.distillation_loss(y := z.clone().requires_grad_(), values, indices, rest), y)
     one = torch.ones((), device=dev)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        loss = bde.distillation_loss(x, values, indices, rest)
-        torch.autograd.grad(loss, x, one, retain_graph=True)
+        x = z.clone().requires_grad_()                 # (a leaf of this stream's: its graph is the only one that is alive)
         loss = bde.distillation_loss(x, values, indices, rest)
         s.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=s):
             (g,) = torch.autograd.grad(loss, x, one, retain_graph=True)
     torch.cuda.current_stream().wait_stream(s)
-    (want,) = torch.autograd.grad(bde.distillation_loss(x, values, indices, rest), x)
     for _ in range(3):
         g.fill_(7.0)
         graph.replay()
@@ -288,3 +304,21 @@ def test_offsets_beyond_32_bits():
     want = bde.distillation_loss(y, values[:1].expand(2, 8), indices[:1].expand(2, 8), rest[:1].expand(2), weight=weight[-2:])
     (gy,) = torch.autograd.grad(want, y)
     assert torch.equal(loss, want) and torch.equal(gz[-2:], gy) and int(torch.count_nonzero(gz[:-2])) == 0
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_takes():
+    """Row-wise kernels split very long batches over launches: rows on both sides of the border."""
+    ops, dev = _hip(), "cuda:0"
+    n, border = (1 << 21) + 5, 1 << 21
+    z, values, indices, rest = (t.to(dev) for t in teacher(8, 12, 3, BF16, 4))
+    pick = (torch.arange(n, device=dev) * 5) % 8
+    x = z[pick].requires_grad_()
+    rows = bde.distillation_loss(x, values[pick], indices[pick], rest[pick], reduction="none")
+    (gx,) = torch.autograd.grad(rows.sum(), x)
+    y = z.clone().requires_grad_()
+    want = bde.distillation_loss(y, values, indices, rest, reduction="none")
+    (gy,) = torch.autograd.grad(want.sum(), y)
+    assert torch.equal(rows, want[pick]) and torch.equal(gx, gy[pick])
+    top, small = bde.topk_logits(x, 3), bde.topk_logits(z, 3)
+    assert torch.equal(top.indices, small.indices[pick]) and torch.equal(top.rest[border - 8:], small.rest[pick[border - 8:]])
