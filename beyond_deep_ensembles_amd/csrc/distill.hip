@@ -160,14 +160,15 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
   const float c = a.inv_tau * kLog2e;
   const float rest = a.rest ? a.rest[row] : neg_inf();
   if (wave == 0) {               // the teacher's largest exponent (natural units) and its sum relative to it
-    float t_top = neg_inf(), bad = rest == neg_inf() ? 0.0f : rest - rest;    // NaN: a NaN or +inf among the teacher's numbers
+    float t_top = neg_inf();
+    bool bad = rest - rest != 0.0f && rest != neg_inf();          // a NaN or +inf among the teacher's numbers
     for (int j = lane; j < a.K; j += 64) {
       const float t = t_l[j];
       t_top = fmaxf(t_top, t);
-      if (t != neg_inf()) bad += t - t;
+      bad = bad || (t - t != 0.0f && t != neg_inf());
     }
     t_top = wave_all_max(t_top);
-    bad = wave_all_sum(bad);
+    bad = __ballot(bad) != 0;
     const float ref = t_top > neg_inf() ? t_top : 0.0f;
     float sum = 0.0f;
     for (int j = lane; j < a.K; j += 64) sum += exp2_hw((t_l[j] - ref) * c);
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
       const float gap = rest - ref * a.inv_tau;
       const float own = t_top > neg_inf() ? kLn2 * __builtin_amdgcn_logf(sum) : neg_inf(), hi = fmaxf(own, gap);
       teacher[0] = ref;
-      teacher[1] = bad != 0.0f ? __builtin_nanf("")
+      teacher[1] = bad                ? __builtin_nanf("")
                    : hi == neg_inf() ? hi        // the teacher says nothing about this row
                                      : hi + kLn2 * __builtin_amdgcn_logf(exp2_hw((own - hi) * kLog2e) + exp2_hw((gap - hi) * kLog2e));
       teacher[2] = gap;
@@ -233,26 +234,25 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
     }
   }
   // the student's listed classes, each counted once: a part per wave that has entries
+  float l_top = neg_inf(), l_sum = 0.0f;
   if (wave * 64 < a.K) {
     if (tid < a.K) z_l[tid] = static_cast<float>(own_z);
-    float l_top = neg_inf();
     for (int j = tid; j < a.K; j += NT) l_top = fmaxf(l_top, z_l[j]);
     l_top = wave_all_max(l_top);
     const float l_ref = l_top > neg_inf() ? l_top : 0.0f;
-    float sum = 0.0f;
     for (int j = tid; j < a.K; j += NT) {
       bool first = v_l[j] >= 0;
       if (dup)
         for (int i = 0; i < j; ++i) first = first && v_l[i] != v_l[j];
-      if (first) sum += exp2_hw((z_l[j] - l_ref) * c);
+      if (first) l_sum += exp2_hw((z_l[j] - l_ref) * c);
     }
-    sum = wave_all_sum(sum);
-    if (lane == 0) {
+    l_sum = wave_all_sum(l_sum);
+    if (W > 1 && lane == 0) {
       listed[2 * wave] = l_top;
-      listed[2 * wave + 1] = sum;
+      listed[2 * wave + 1] = l_sum;
     }
   }
-  if (lane == 0) {
+  if (W > 1 && lane == 0) {
     others[2 * wave] = ref;
     others[2 * wave + 1] = tail;
   }
@@ -266,9 +266,11 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
   };
   const float t_ref = teacher[0], t_log = teacher[1], r_log = teacher[2] - t_log, r = rest > neg_inf() ? exp2_hw(r_log * kLog2e) : 0.0f;
   const bool silent = t_log == neg_inf();
-  float other, l_top, l_sum;
-  join(others, W, other, tail);
-  join(listed, min(W, (a.K + 63) >> 6), l_top, l_sum);
+  float other = ref;
+  if constexpr (W > 1) {
+    join(others, W, other, tail);
+    join(listed, min(W, (a.K + 63) >> 6), l_top, l_sum);
+  }
   const float top = fmaxf(other, l_top);
   const float o_scale = exp2_hw((other - top) * c);
   const float sum = tail * o_scale + (l_top > neg_inf() ? l_sum * exp2_hw((l_top - top) * c) : 0.0f);
@@ -328,7 +330,13 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
 __global__ __launch_bounds__(1024) void distill_inv_weight_kernel(const float* weight, int n, float* inv) {
   __shared__ double smem[16];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) s += weight[i];
+  for (int i = threadIdx.x; i < n; i += 4096) {       // four loads in flight
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = i + 1024 * u < n ? weight[i + 1024 * u] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s += x[u];
+  }
   s = block_sum(s, smem);
   if (threadIdx.x == 0) *inv = s != 0.0 ? static_cast<float>(1.0 / s) : 0.0f;
 }
@@ -336,7 +344,13 @@ __global__ __launch_bounds__(1024) void distill_inv_weight_kernel(const float* w
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* loss, int n, float* out) {
   __shared__ double smem[16];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) s += loss[i];
+  for (int i = threadIdx.x; i < n; i += 4096) {       // four loads in flight
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = i + 1024 * u < n ? loss[i + 1024 * u] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s += x[u];
+  }
   s = block_sum(s, smem);
   if (threadIdx.x == 0) *out = static_cast<float>(s);
 }
