@@ -175,7 +175,8 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
     sum = wave_all_sum(sum);
     if (lane == 0) {
       // log of the whole, relative to ref: log(sum + e^(rest - ref / tau)), from the larger of the two
-      const float gap = rest - ref * a.inv_tau;
+      // (a list of the type's lowest value, a mask, may leave the range at a temperature below 1)
+      const float gap = rest > neg_inf() ? fminf(rest - ref * a.inv_tau, 3.0e38f) : neg_inf();
       const float own = t_top > neg_inf() ? kLn2 * __builtin_amdgcn_logf(sum) : neg_inf(), hi = fmaxf(own, gap);
       teacher[0] = ref;
       teacher[1] = bad                ? __builtin_nanf("")
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
 __global__ __launch_bounds__(1024) void distill_inv_weight_kernel(const float* weight, int n, float* inv) {
   __shared__ double smem[16];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 4096) {       // four loads in flight
+  for (int64_t i = threadIdx.x; i < n; i += 4096) {       // four loads in flight
     float x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) x[u] = i + 1024 * u < n ? weight[i + 1024 * u] : 0.0f;
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(1024) void distill_inv_weight_kernel(const float* w
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* loss, int n, float* out) {
   __shared__ double smem[16];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 4096) {       // four loads in flight
+  for (int64_t i = threadIdx.x; i < n; i += 4096) {       // four loads in flight
     float x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) x[u] = i + 1024 * u < n ? loss[i + 1024 * u] : 0.0f;

@@ -486,6 +486,16 @@ def test_distill_lists_with_structure(backend, v, k):
     check_distill(backend, z, values, indices, rest)
 
 
+@pytest.mark.parametrize("tau", [0.6, 1.0, 2.0])
+def test_distill_teachers_masked_with_the_lowest_value(backend, tau):
+    """A teacher whose list holds nothing but the type's lowest value: alone it is uniform over the list, beside a finite rest
+    nothing."""
+    z, values, indices, rest = teacher(4, 40, 5, F32, 7, tau)
+    values[:] = torch.finfo(F32).min
+    rest[:2] = -math.inf
+    check_distill(backend, z, values, indices, rest, tau=tau)
+
+
 @pytest.mark.parametrize("v,spike", [(3000, 2900), (20001, 19990), (70000, 69000)])
 def test_distill_rows_that_rise_late(backend, v, spike):
     """The largest classes lie behind each thread's first granule, so far above it that the provisional reference overflows; and
