@@ -202,6 +202,8 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
   }
   row_sync<NT>();
   int n = n_hit <= kCap ? n_cand : kCap + 1;
+  uint32_t key = bound;                                 // when exactly k are listed: they lie above it, or on it up to class v_hi
+  int v_hi = a.V - 1;
   if (n > kCap) {
     // Too many elements reach the bound (they are equal, or nearly all of the row is): the k-th largest key itself, then the
     // class up to which the elements equal to it belong.  Counts over the row, read again.
@@ -219,7 +221,6 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
       }
       return row_count<NT>(m, counts);
     };
-    uint32_t key = bound;
     if (count(key, -1) >= a.K) {
       uint32_t lo = key + 1u, hi = 0xFFFFFFFFu;         // invariant: count(>= lo) >= k, count(> hi) < k
       while (lo < hi) {
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
       }
       key = lo;
     }
-    int v_lo = -1, v_hi = a.V - 1;                      // invariant: too few with v <= v_lo, enough with v <= v_hi
+    int v_lo = -1;                                      // invariant: too few with v <= v_lo, enough with v <= v_hi
     while (v_hi - v_lo > 1) {
       const int mid = v_lo + ((v_hi - v_lo) >> 1);
       if (count(key, mid) >= a.K) v_hi = mid;
@@ -272,6 +273,28 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
       for (int j = 0; j < n; ++j) rank[q] += cand[j] > mine[q] ? 1 : 0;
   }
   others = row_all_sum<NT>(others, slots);   // (its barrier: the list has been read)
+  if (a.rest && n == a.K && n < a.V && !(others >= 1.0e-20f && others < __builtin_inff())) {
+    // The selected elements are infinite, or so far above the others that those vanish beside them: the others' sum relative to
+    // the largest of them, over the row read again.
+    auto over_others = [&](auto f) {
+      for (int g = tid; g < z.granules; g += NT) {
+        const u32x4 x = z.load(g);
+        const int e0 = z.first(g);
+        for (int i = 0; i < GN; ++i) {
+          const int v = e0 + i;
+          const float e = granule_get<T>(x, i);
+          const uint32_t k = order_key(e);
+          if (v >= 0 && v < a.V && (k < key || (k == key && v > v_hi))) f(e);
+        }
+      }
+    };
+    float m = neg_inf(), sum = 0.0f;
+    over_others([&](float e) { m = fmaxf(m, e); });
+    m = row_all_max<NT>(m, slots + W);
+    ref = m - m == 0.0f ? m : 0.0f;
+    over_others([&](float e) { sum += exp2_hw((e - ref) * c); });
+    others = row_all_sum<NT>(sum, slots);
+  }
 #pragma unroll
   for (int q = 0; q < kMine; ++q) {
     if (tid + q * NT >= n) continue;
@@ -299,8 +322,8 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void topk_logits_kernel(Top
   more = row_all_sum<NT>(more, slots + W);
   if (tid == 0) {
     float r = neg_inf();
-    if (left > 0 && more != 0.0f)              // ref <= from: the others' sum relative to it
-      r = from * a.inv_tau + kLn2 * __builtin_amdgcn_logf(more + others * exp2_hw((ref - from) * c));
+    if (left > 0 && more != 0.0f)              // ref <= from where anything lies below the bound: the others' sum relative to it
+      r = from * a.inv_tau + kLn2 * __builtin_amdgcn_logf(more + (others != 0.0f ? others * exp2_hw((ref - from) * c) : 0.0f));
     else if (others != 0.0f)
       r = ref * a.inv_tau + kLn2 * __builtin_amdgcn_logf(others);
     a.rest[row] = r;

@@ -337,6 +337,33 @@ def test_topk_rows_with_structure(backend, row, v, k):
     check_topk(backend, z, k)
 
 
+@pytest.mark.parametrize("top", [math.inf, math.nan, None])
+@pytest.mark.parametrize("v,k", [(50, 1), (50, 30), (3001, 3), (3001, 200)])
+def test_topk_what_is_left_beside_infinities(backend, v, k, top):
+    """Exactly k classes that are +inf (NaN): the others are summed relative to a number of their own, also where their
+    exponentials leave the range, and so small that they would vanish.  (None: the same rows without them.)"""
+    z = torch.randn(3, v, generator=gen(v + k)) + torch.tensor([[200.0], [-300.0], [0.0]])
+    if top is not None:
+        z[:, torch.randperm(v, generator=gen(k))[:k]] = top
+    check_topk(backend, z, k)
+
+
+@pytest.mark.parametrize("gap", [40.0, 100.0, 150.0, 1e4, 1e30])
+@pytest.mark.parametrize("v,k", [(50, 1), (50, 30), (3001, 3), (3001, 200)])
+def test_topk_what_is_left_far_below(backend, v, k, gap):
+    """Exactly k classes that lie far above the others: what is left is still the others' sum, not nothing."""
+    z = torch.randn(2, v, generator=gen(v + k))
+    z[:, torch.randperm(v, generator=gen(k))[:k]] += gap
+    ops, dev = backend
+    got = bde.topk_logits(z.to(dev), k, _ops=ops)
+    values, indices, rest = topk64(z, k, 1.0)
+    assert torch.equal(got.indices.cpu(), indices)
+    close(got.values, values, 0.0, "values")
+    # relative to the k-th value the difference (one rounding of up to gap + 8) is an error of the exponent, below 1e-20 of a sum
+    # relative to the largest of the others none
+    close(got.rest, rest, exponent_error(min(gap, 60.0) + 16, v) + 4 * U * (gap if gap <= 60 else 16.0), "rest")
+
+
 def test_topk_strided_rows(backend):
     wide = torch.randn(4, 700, generator=gen(4))
     for z in (wide[:, :301], wide[:, 3:302], wide[::2, 1:400], wide.t()[:90], wide[:1].expand(3, 700)):
