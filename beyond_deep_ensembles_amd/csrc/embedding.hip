@@ -47,6 +47,7 @@ struct EmbedArgs {
   int* dealt_p;            // [N] positions by group, in order
   int* dealt_t;            // [N] their tokens
   int stream_zeros;        // zero rows are stored past the caches
+  int join0;               // first workgroup of this launch of the join
 };
 
 // VEC consecutive elements as fp32
@@ -501,9 +502,9 @@ template <typename TW, int NOISE, int VEC>
 __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(EmbedArgs a, int column_tiles) {
   constexpr int NACC = NOISE == kNoisePosition ? 2 : 1, kWaves = kJoinBlock / 64;
   __shared__ float sums[kWaves - 1][NACC][64 * VEC];
-  const int piece = static_cast<int>(blockIdx.x) / column_tiles;
+  const int id = a.join0 + static_cast<int>(blockIdx.x), piece = id / column_tiles;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int d = (static_cast<int>(blockIdx.x) % column_tiles) * 64 * VEC + lane * VEC;
+  const int d = (id % column_tiles) * 64 * VEC + lane * VEC;
   const int n = a.header[0], s0 = piece * a.piece, s1 = s0 + a.piece;
   if (s1 >= n) return;
   const int key = a.key[s1 - 1];
@@ -585,8 +586,9 @@ static int embedding_fwd_launch(const EmbedArgs& a, hipStream_t s) {
   if (a.N >= kFwdManyRows) return go(&embedding_fwd_kernel<TW, TO, NOISE, VEC, 4>, 4);
   return go(&embedding_fwd_kernel<TW, TO, NOISE, VEC, 1>, 1);
 }
+constexpr int kJoinsPerLaunch = 1 << 19;       // (a launch holds fewer than 2^32 threads)
 template <typename TW, typename TG, int NOISE, int VEC>
-static int embedding_bwd_launch(const EmbedArgs& a, hipStream_t s) {
+static int embedding_bwd_launch(EmbedArgs a, hipStream_t s) {
   const dim3 groups(1u << a.log_groups);
   const size_t lds = sizeof(int) * kSortWaves * a.bucket;
   if (a.chunk > 0) {
@@ -602,11 +604,17 @@ static int embedding_bwd_launch(const EmbedArgs& a, hipStream_t s) {
   if (const int rc = to_err(hipGetLastError())) return rc;
   if (a.N == 0) return 0;
   const int tiles = (a.D + 64 * VEC - 1) / (64 * VEC), pieces = static_cast<int>((a.N + a.piece - 1) / a.piece);
-  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(pieces) * tiles + kBlock / 64 - 1) / (kBlock / 64));
-  hipLaunchKernelGGL((embedding_sum_kernel<TW, TG, NOISE, VEC>), dim3(blocks), dim3(kBlock), 0, s, a, tiles);
+  const int64_t all = static_cast<int64_t>(pieces) * tiles;
+  hipLaunchKernelGGL((embedding_sum_kernel<TW, TG, NOISE, VEC>), dim3(static_cast<unsigned>((all + kBlock / 64 - 1) / (kBlock / 64))), dim3(kBlock), 0, s,
+                     a, tiles);
   if (const int rc = to_err(hipGetLastError())) return rc;
-  if (pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<TW, NOISE, VEC>), dim3(pieces * tiles), dim3(kJoinBlock), 0, s, a, tiles);
-  return to_err(hipGetLastError());
+  for (int64_t first = 0; pieces > 1 && first < all; first += kJoinsPerLaunch) {
+    a.join0 = static_cast<int>(first);
+    const unsigned joins = static_cast<unsigned>(std::min<int64_t>(kJoinsPerLaunch, all - first));
+    hipLaunchKernelGGL((embedding_join_kernel<TW, NOISE, VEC>), dim3(joins), dim3(kJoinBlock), 0, s, a, tiles);
+    if (const int rc = to_err(hipGetLastError())) return rc;
+  }
+  return 0;
 }
 
 static bool on_border(const void* p, int64_t ld, size_t element, int vec) {

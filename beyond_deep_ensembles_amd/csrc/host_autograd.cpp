@@ -275,7 +275,7 @@ template <typename... Args>
 }
 int type_code(at::ScalarType t) { return t == at::kFloat ? BDE_F32 : t == at::kBFloat16 ? BDE_BF16 : t == at::kHalf ? BDE_F16 : -1; }
 void need_device(const at::Tensor& t, const char* name) {
-  const bool there = t.is_cuda() && true;
+  const bool there = t.is_cuda() && t.layout() == at::kStrided;
   if (!there)
     refuse(name, ": expected a CUDA (HIP) tensor, got device ", t.device().str(), "; beyond_deep_ensembles_amd has no CPU path");
 }

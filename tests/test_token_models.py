@@ -322,3 +322,17 @@ def test_more_rows_than_one_launch_takes():
     assert torch.equal(rows, want[pick]) and torch.equal(gx, gy[pick])
     top, small = bde.topk_logits(x, 3), bde.topk_logits(z, 3)
     assert torch.equal(top.indices, small.indices[pick]) and torch.equal(top.rest[border - 8:], small.rest[pick[border - 8:]])
+
+
+@pytest.mark.gpu
+def test_embedding_gradient_of_more_joins_than_one_launch_takes():
+    """Two million positions of an odd width: the joins of runs that cross pieces take two launches.  All rows of the gradient
+    are one row, so the sums are whole multiples of it: exact."""
+    ops, dev = _hip(), "cuda:0"
+    n, d = (1 << 21) + 6400, 1001
+    tokens = (torch.arange(n, device=dev) % 6).int()
+    tokens[-6000:] = 6                                           # a run that begins behind the border
+    row = (torch.arange(d, device=dev) % 5 - 2).float().bfloat16()
+    grad = torch.empty(7, d, device=dev)
+    ops.embedding_bwd(row.expand(n, d), tokens, grad)
+    assert torch.equal(grad, torch.bincount(tokens, minlength=7).float()[:, None] * row.float())
