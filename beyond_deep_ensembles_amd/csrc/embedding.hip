@@ -253,6 +253,27 @@ __global__ __launch_bounds__(kSortThreads) void embedding_deal_kernel(EmbedArgs 
   }
 }
 
+// the gradient rows of a token that does not occur, by one wave
+__device__ __forceinline__ void zero_row(const EmbedArgs& a, char* p, int64_t bytes, int lane) {
+  if (bytes % 16 == 0) {
+    const u32x4 z = {0u, 0u, 0u, 0u};
+    if (a.stream_zeros)
+      for (int64_t b = lane * 16; b < bytes; b += 1024) __builtin_nontemporal_store(z, reinterpret_cast<u32x4*>(p + b));
+    else
+      for (int64_t b = lane * 16; b < bytes; b += 1024) *reinterpret_cast<u32x4*>(p + b) = z;
+  } else if (bytes % 4 == 0) {
+    for (int64_t b = lane * 4; b < bytes; b += 256) *reinterpret_cast<uint32_t*>(p + b) = 0u;
+  } else {
+    for (int64_t b = lane * 2; b < bytes; b += 128) *reinterpret_cast<uint16_t*>(p + b) = 0;
+  }
+}
+template <typename TW>
+__device__ __forceinline__ void zero_token(const EmbedArgs& a, int64_t t, int lane) {
+  const int64_t row_bytes = static_cast<int64_t>(a.D) * sizeof(TW);
+  zero_row(a, static_cast<char*>(a.gw) + t * row_bytes, row_bytes, lane);
+  if (a.grho) zero_row(a, reinterpret_cast<char*>(a.grho) + t * a.D * 4, static_cast<int64_t>(a.D) * 4, lane);
+}
+
 template <typename TW, bool DEALT>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs a, int log_groups) {
   extern __shared__ int hist[];                     // [16][bucket] counts, then where the next one goes
@@ -385,27 +406,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
     });
   }
   place_list(listed);
-  // rows of tokens that do not occur: zero
-  const int64_t row_bytes = static_cast<int64_t>(a.D) * sizeof(TW);
-  auto zero_row = [&](char* p, int64_t bytes) {
-    if (bytes % 16 == 0) {
-      const u32x4 z = {0u, 0u, 0u, 0u};
-      if (a.stream_zeros)
-        for (int64_t b = lane * 16; b < bytes; b += 1024) __builtin_nontemporal_store(z, reinterpret_cast<u32x4*>(p + b));
-      else
-        for (int64_t b = lane * 16; b < bytes; b += 1024) *reinterpret_cast<u32x4*>(p + b) = z;
-    } else if (bytes % 4 == 0) {
-      for (int64_t b = lane * 4; b < bytes; b += 256) *reinterpret_cast<uint32_t*>(p + b) = 0u;
-    } else {
-      for (int64_t b = lane * 2; b < bytes; b += 128) *reinterpret_cast<uint16_t*>(p + b) = 0;
-    }
-  };
-  for (int r = wave; r < own; r += kSortWaves) {
-    if (totals[r]) continue;
-    const int64_t t = (static_cast<int64_t>(r) << log_groups) + group;
-    zero_row(static_cast<char*>(a.gw) + t * row_bytes, row_bytes);
-    if (a.grho) zero_row(reinterpret_cast<char*>(a.grho) + t * a.D * 4, static_cast<int64_t>(a.D) * 4);
-  }
+  for (int r = wave; r < own; r += kSortWaves)
+    if (!totals[r]) zero_token<TW>(a, (static_cast<int64_t>(r) << log_groups) + group, lane);
 }
 
 // the sums of one token's run -> its gradient rows
@@ -555,6 +557,139 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(EmbedArgs a,
   embedding_finish<TW, NOISE, VEC>(a, key, d, acc, acc2);
 }
 
+// ---- few positions: the whole gradient in ONE launch
+// Workgroup b owns the tokens it owns in the sort; it collects its positions in LDS as (token, position), ranks them by counting
+// and adds the rows in that order: eight waves take consecutive pieces of the list, the parts of runs that cross pieces are
+// added in order.  Nothing passes through memory, and the host, which bounds calls this small, launches once.
+// What bounds the kernel are its zero rows, or one workgroup that owns most positions and reads most of g alone -- hence the
+// limits.  Positions by word frequency / half of them one token / all of them, against the several launches: 64 x 256 bf16,
+// 1,000 tokens 3.8 / 5.7 / 6.6 us against 11.9 / 11.9 / 11.1; 512 x 256 6.3 / 13.9 / 25.3 against 13.1 / 13.8 / 12.8; 512 x 256
+// fp32, 30,011 tokens 9.5 / 19.8 / 31.7 against 16.2 / 17.2 / 15.5; beyond: 512 x 1,024 27 / 66 / 105 against 28 / 28 / 27.
+constexpr int kSmallTokens = 512, kSmallThreads = 512, kSmallWaves = kSmallThreads / 64;
+constexpr int64_t kSmallElements = 128 << 10;
+static bool embedding_small(int64_t n, int64_t d) { return n <= kSmallTokens && n * d <= kSmallElements; }
+
+template <typename TW, typename TG, int NOISE, int VEC>
+__global__ __launch_bounds__(kSmallThreads) void embedding_small_kernel(EmbedArgs a, int log_groups) {
+  constexpr int NACC = NOISE == kNoisePosition ? 2 : 1, kAhead = 8;
+  static_assert(kSmallTokens <= kSmallThreads && kSmallTokens <= 1 << 10 && kSmallTokens % 16 == 0, "a thread per position; ten bits of an entry");
+  __shared__ __attribute__((aligned(16))) uint32_t found[kSmallTokens], list[kSmallTokens];
+  __shared__ uint32_t seen[kMaxBucket / 32];
+  __shared__ float part[kSmallWaves][2][NACC][64 * VEC];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = static_cast<int>(blockIdx.x), groups = 1 << log_groups, n = static_cast<int>(a.N);
+  const int own = group < a.V ? (a.V - group + groups - 1) >> log_groups : 0;
+  const int64_t raw = tid < n ? raw_token(a, tid) : -1;
+  if (tid < kMaxBucket / 32) seen[tid] = 0u;
+  if (tid < kSmallTokens) found[tid] = ~0u;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  const int t = static_cast<int>(raw);
+  if (live_token(a, raw) && (t & (groups - 1)) == group) {
+    const int r = t >> log_groups;
+    found[atomicAdd(&count, 1)] = static_cast<uint32_t>(r) << 10 | static_cast<uint32_t>(tid);
+    atomicOr(&seen[r >> 5], 1u << (r & 31));
+  }
+  __syncthreads();
+  const int m = __builtin_amdgcn_readfirstlane(count);
+  if (tid < m) {
+    const uint32_t mine = found[tid];                   // (the entries are all different, what is behind them is larger)
+    int rank = 0;
+    for (int j = 0; j < m; j += 16) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(found + j + 4 * q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rank += x[k] < mine ? 1 : 0;
+      }
+    }
+    list[rank] = mine;
+  }
+  __syncthreads();
+  auto entry_token = [](int entry) { return static_cast<int>(static_cast<uint32_t>(entry) >> 10); };
+  auto token = [&](int i) { return __builtin_amdgcn_readfirstlane(i >= 0 && i < m ? entry_token(static_cast<int>(list[i])) : -1); };
+  float acc[VEC], acc2[VEC];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = acc2[i] = 0.0f;
+  };
+  const int tiles = (a.D + 64 * VEC - 1) / (64 * VEC);
+  const bool alone = m <= kAhead;                        // one piece: the waves take the columns
+  const int piece = max(kAhead, (m + kSmallWaves - 1) / kSmallWaves);
+  const int begin = alone ? 0 : min(m, wave * piece), end = min(m, begin + piece);
+  for (int c = alone ? wave : 0; c < tiles; c += alone ? kSmallWaves : 1) {
+    const int d = c * 64 * VEC + lane * VEC;
+    const bool active = d < a.D;
+    // entries [begin, end) of the list: finished runs are stored, the parts of others kept
+    clear();
+    int run_begin = begin;
+    const int before = token(begin - 1);
+    for (int s = begin; s < end; s += kAhead) {
+      const uint32_t mine = lane <= kAhead && s + lane < m ? list[s + lane] : ~0u;      // (one more: the entry behind)
+      float g[kAhead][VEC], e[NACC == 2 ? kAhead : 1][VEC];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s + u < end) {
+          const int64_t pos = __builtin_amdgcn_readlane(static_cast<int>(mine), u) & 1023;
+          if (active) {
+            load_vec<TG, VEC>(static_cast<const TG*>(a.g) + pos * a.ldg + d, g[u]);
+            if constexpr (NACC == 2) {
+              if (a.eps) load_vec<float, VEC>(a.eps + pos * a.ldeps + d, e[u]);
+              else noise_vec<VEC>(a.seed, a.stream_id, pos * a.D + d, e[u]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s + u < end) {
+          const int r = entry_token(__builtin_amdgcn_readlane(static_cast<int>(mine), u));
+          const int next = entry_token(__builtin_amdgcn_readlane(static_cast<int>(mine), u + 1));
+          if (active) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              acc[i] += g[u][i];
+              if constexpr (NACC == 2) acc2[i] = __builtin_fmaf(g[u][i], e[u][i], acc2[i]);
+            }
+          }
+          if (next != r || s + u + 1 == end) {
+            const bool begun_before = run_begin == begin && before == r;
+            if (begun_before || next == r) {
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                part[wave][begun_before ? 0 : 1][0][i * 64 + lane] = acc[i];
+                if constexpr (NACC == 2) part[wave][begun_before ? 0 : 1][NACC - 1][i * 64 + lane] = acc2[i];
+              }
+            } else if (active) {
+              embedding_finish<TW, NOISE, VEC>(a, (r << log_groups) + group, d, acc, acc2);
+            }
+            clear();
+            run_begin = s + u + 1;
+          }
+        }
+      }
+    }
+    if (alone) continue;
+    __syncthreads();
+    // the wave in whose piece a run begins that goes on behind it
+    const int r = token(end - 1);
+    if (begin < end && end < m && token(end) == r && (begin == 0 || token(begin - 1) != r || token(begin) != r)) {
+      clear();
+      for (int w = wave; w < kSmallWaves && w * piece < m && (w == wave || token(w * piece) == r); ++w)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          acc[i] += part[w][w == wave ? 1 : 0][0][i * 64 + lane];
+          if constexpr (NACC == 2) acc2[i] += part[w][w == wave ? 1 : 0][NACC - 1][i * 64 + lane];
+        }
+      if (active) embedding_finish<TW, NOISE, VEC>(a, (r << log_groups) + group, d, acc, acc2);
+    }
+    __syncthreads();
+  }
+  for (int r = wave; r < own; r += kSmallWaves)
+    if (!((seen[r >> 5] >> (r & 31)) & 1u)) zero_token<TW>(a, (static_cast<int64_t>(r) << log_groups) + group, lane);
+}
+
 constexpr int64_t kDealTokens = 49152;
 // positions per workgroup of the dealing kernels (0: no dealing): at most 256 chunks, whole waves of 64 positions
 static int embedding_chunk(int64_t n) {
@@ -590,6 +725,10 @@ constexpr int kJoinsPerLaunch = 1 << 19;       // (a launch holds fewer than 2^3
 template <typename TW, typename TG, int NOISE, int VEC>
 static int embedding_bwd_launch(EmbedArgs a, hipStream_t s) {
   const dim3 groups(1u << a.log_groups);
+  if (embedding_small(a.N, a.D)) {
+    hipLaunchKernelGGL((embedding_small_kernel<TW, TG, NOISE, VEC>), groups, dim3(kSmallThreads), 0, s, a, a.log_groups);
+    return to_err(hipGetLastError());
+  }
   const size_t lds = sizeof(int) * kSortWaves * a.bucket;
   if (a.chunk > 0) {
     const int chunks = static_cast<int>((a.N + a.chunk - 1) / a.chunk);
@@ -602,7 +741,6 @@ static int embedding_bwd_launch(EmbedArgs a, hipStream_t s) {
     hipLaunchKernelGGL((embedding_sort_kernel<TW, false>), groups, dim3(kSortThreads), lds, s, a, a.log_groups);
   }
   if (const int rc = to_err(hipGetLastError())) return rc;
-  if (a.N == 0) return 0;
   const int tiles = (a.D + 64 * VEC - 1) / (64 * VEC), pieces = static_cast<int>((a.N + a.piece - 1) / a.piece);
   const int64_t all = static_cast<int64_t>(pieces) * tiles;
   hipLaunchKernelGGL((embedding_sum_kernel<TW, TG, NOISE, VEC>), dim3(static_cast<unsigned>((all + kBlock / 64 - 1) / (kBlock / 64))), dim3(kBlock), 0, s,
@@ -678,6 +816,7 @@ constexpr int64_t kDealBytes = 4 * (256 * kMaxDealGroups + kMaxDealGroups + 64);
 
 extern "C" size_t bde_embedding_bwd_ws_bytes(int64_t N, int64_t D, int noise) {
   if (N < 0 || N > BDE_EMBEDDING_MAX_TOKENS || D < 1 || D > BDE_EMBEDDING_MAX_DIM) return 0;
+  if (embedding_small(N, D)) return 256;      // (not used)
   const int64_t list = (4 * N + 255) / 256 * 256;
   const int64_t lists = 256 + 2 * list + (embedding_chunk(N) > 0 ? 2 * list + kDealBytes : 0);
   const int64_t pieces = (N + embedding_piece(N) - 1) / embedding_piece(N);

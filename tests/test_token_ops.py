@@ -140,6 +140,37 @@ def test_embedding_token_patterns(backend, tokens):
     check_embedding(backend, t, w, rho, noise="position", eps=torch.randn(tuple(t.shape) + (d,), generator=g), pad=pad)
 
 
+@pytest.mark.parametrize("wtype,otype", TYPES, ids=[f"{NAMES[a]}-{NAMES[b]}" for a, b in TYPES])
+@pytest.mark.parametrize("n,v,d", [(9, 1, 8), (64, 2, 301), (200, 5, 520), (512, 3, 4), (513, 300, 6), (300, 7, 904)])
+def test_embedding_gradient_in_one_launch_and_in_several(backend, n, v, d, wtype, otype):
+    """Few positions take one launch, more several: sizes on both sides of the bounds; runs that lie within a wave's piece of the
+    list, cross one border, or hold whole pieces; columns in several tiles."""
+    g = gen(n + d)
+    tokens = (v * torch.rand(n, generator=g) ** 2).long()
+    check_embedding(backend, tokens, torch.randn(v, d, generator=g).to(wtype), None, scale=0.5, out_dtype=otype)
+
+
+@pytest.mark.parametrize("noise", ["position", "token"])
+@pytest.mark.parametrize("n,v,d", [(90, 3, 264), (90, 3, 67), (520, 4, 8), (300, 40, 900)])
+def test_gaussian_embedding_gradient_in_one_launch_and_in_several(backend, n, v, d, noise):
+    g = gen(n + d)
+    tokens = (v * torch.rand(n, generator=g) ** 2).long()
+    mean, rho = torch.randn(v, d, generator=g), torch.randn(v, d, generator=g) - 2
+    check_embedding(backend, tokens, mean, rho, noise=noise, eps=torch.randn(n if noise == "position" else v, d, generator=g), pad=1)
+
+
+@pytest.mark.parametrize("tokens", ["one", "two", "falling", "padding_only", "outside"])
+def test_embedding_token_patterns_of_many_positions(backend, tokens):
+    v, d, pad, n = 11, 12, 2, 1056
+    i = torch.arange(n)
+    t = {"one": torch.full((n,), 4), "two": torch.where(i % 2 == 0, 9, 1), "falling": 10 - i // 96, "padding_only": torch.full((n,), pad),
+         "outside": torch.tensor([3, -1, 11, 3, 2, -2 ** 40, 2 ** 40, 10]).repeat(n // 8)}[tokens]
+    g = gen(8)
+    w, rho = torch.randn(v, d, generator=g), torch.randn(v, d, generator=g) - 2
+    check_embedding(backend, t, w, None, scale=3.0, pad=pad)
+    check_embedding(backend, t, w, rho, noise="position", eps=torch.randn(n, d, generator=g), pad=pad)
+
+
 @pytest.mark.parametrize("noise", ["position", "token"])
 @pytest.mark.parametrize("otype", [F32, BF16, F16], ids=lambda t: NAMES[t])
 @pytest.mark.parametrize("n,v,d", [(50, 9, 16), (70, 300, 13)])

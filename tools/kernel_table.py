@@ -114,6 +114,7 @@ ROWS = {
     "embedding_sort_kernel": ("positions sorted by token in one launch; zero rows of absent tokens", "`8·N` B + the absent rows", "47 µs with 235 MB of zero rows; 17.8 µs with 86 MB; `token_ops_kernel_times.txt`", TOK, "same"),
     "embedding_count_kernel": ("many tokens: how many of each chunk go to each workgroup of the sort", "`8·N` B", "4.8 µs at 65,536 tokens; `token_ops_kernel_times.txt`", TOK, "`test_embedding_gradient_of_many_tokens`"),
     "embedding_deal_kernel": ("many tokens: positions dealt out to the sort's workgroups, in order", "`16·N` B", "8.5 µs at 65,536 tokens; `token_ops_kernel_times.txt`", TOK, "same test"),
+    "embedding_small_kernel": ("the whole gradient of at most 512 positions in one launch", "`N·D` in, `V·D` out", "3.8 µs at 64 × 256 bf16, 1,000 rows; 9.5 µs at 512 × 256 fp32, 30,011 rows", TOK, "same"),
     "embedding_sum_kernel": ("the tokens' gradient rows, added in order (torch: atomics)", "`N·D` in, touched rows out", "46 µs at 65,536 × 1,024 bf16 (30 µs with warm inputs); `token_ops_kernel_times.txt`", TOK, "same"),
     "embedding_join_kernel": ("runs that cross a piece of the sorted list", "latency", "8 µs at 65,536 tokens; `token_ops_kernel_times.txt`", TOK, "`test_embedding_token_patterns`"),
     "topk_logits_kernel": ("a teacher's k largest logits, their classes and the log-sum of the rest", "`N·V` read once", "63 µs = 4.2 TB/s at 4,096 × 32,000 bf16, k = 64; `token_ops_kernel_times.txt`", TOK, "`test_topk_*`"),
