@@ -1,5 +1,5 @@
 // Native host helper of the optimizer shells: the per-tensor pointer-aliasing loops in C++ (the layers' autograd
-// nodes live in host_autograd.cpp, same module).
+// nodes live in host_autograd.cpp, the token-model operators' in host_tokens.cpp, same module).
 //
 // The reference re-points `param.data` (and hands over `param.grad`) tensor by tensor in Python
 // (src/algos/svgd.py:93-96,120-127; swag.py:58,81; ivorn.py:111).  With ResNet-50's 161 tensors an
@@ -340,9 +340,11 @@ void small_step_adam(int64_t e_gather, int64_t e_step, at::Tensor seg_ptrs, at::
 }  // namespace
 
 void bind_autograd_nodes(py::module_& m);   // host_autograd.cpp: the Bayesian layers' autograd nodes
+void bind_token_nodes(py::module_& m);      // host_tokens.cpp: the token-model operators'
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_autograd_nodes(m);
+  bind_token_nodes(m);
   py::class_<Layout>(m, "Layout")
       .def(py::init<std::vector<int64_t>, std::vector<int64_t>, std::vector<std::vector<int64_t>>>())
       .def("views", &Layout::views, "per-parameter views of a flat row")

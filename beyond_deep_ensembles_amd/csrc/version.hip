@@ -5,8 +5,6 @@ extern "C" const char* bde_arch(void) { return "gfx950"; }
 extern "C" {
 int bde_internal_load_conv_lrt(void);
 int bde_internal_load_conv_lrt_bwd(void);
-int bde_internal_load_distill(void);
-int bde_internal_load_embedding(void);
 int bde_internal_load_gauss(void);
 int bde_internal_load_ivon(void);
 int bde_internal_load_lrt(void);
@@ -16,7 +14,10 @@ int bde_internal_load_svgd_fused(void);
 int bde_internal_load_svgd_small(void);
 int bde_internal_load_swag(void);
 int bde_internal_load_swag_batched(void);
-int bde_internal_load_topk(void);
+// the token-model operators' files: a library built without them has none to load
+int bde_internal_load_distill(void) __attribute__((weak));
+int bde_internal_load_embedding(void) __attribute__((weak));
+int bde_internal_load_topk(void) __attribute__((weak));
 }
 
 // Load every code object of the library on the CURRENT device.  HIP defers the upload of a code object to the first
@@ -37,6 +38,7 @@ extern "C" int bde_init(void) {
                                    bde_internal_load_svgd,  bde_internal_load_svgd_fused, bde_internal_load_swag, bde_internal_load_swag_batched,
                                    bde_internal_load_embedding, bde_internal_load_topk, bde_internal_load_distill};
   for (auto load : required) {
+    if (!load) continue;
     const int rc = load();
     if (rc) return rc;
   }

@@ -22,7 +22,7 @@ _default = None         # the product's one backend, made at the first call that
 
 
 def _backend(ops):
-    """(the kernel backend, the C++ nodes of lib/_bde_host.so or None): the nodes (csrc/host_autograd.cpp) are what this module's
+    """(the kernel backend, the C++ nodes of lib/_bde_host.so or None): the nodes (csrc/host_tokens.cpp) are what this module's
     Python path does, without its interpreter time; they exist for the HIP library only."""
     global _layers, _default
     if _layers is None:

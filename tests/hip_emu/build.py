@@ -123,10 +123,32 @@ def _build_locked(sources, defines, names, texts, out_dir, lib):
     return lib
 
 
+TOKEN_SOURCES = {"embedding.hip", "topk.hip", "distill.hip"}
+_HELPERS = {            # lines of the host sources that only the device has -> what stands there on the model
+    "void* current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }":
+        "void* current_stream(const at::Tensor&) { return nullptr; }",
+    "#include <c10/hip/HIPStream.h>": "",
+}
+
+
+def _host_source(name):
+    text = open(os.path.join(CSRC, name)).read()
+    assert "t.is_cuda() &&" in text
+    for line, instead in _HELPERS.items():
+        assert line + "\n" in text, (name, line)
+        text = text.replace(line, instead)
+    if name == "host_tokens.cpp":
+        line = next(ln for ln in text.splitlines() if ln.startswith("bool stream_capturing(void* stream)"))
+        text = text.replace(line, "bool stream_capturing(void*) { return false; }")
+    text = text.replace("t.is_cuda() &&", "!t.is_cuda() &&")
+    return text.replace('#include "../../include/bde_hip.h"', f'#include "{os.path.join(ROOT, "include", "bde_hip.h")}"')
+
+
 def build_host_nodes(sources):
     """-> path of `_bde_host_emu.so`: the C++ autograd nodes of csrc/host_autograd.cpp (what lib/_bde_host.so binds for the
-    Bayesian layers) over the CPU model.  The source is used as it is except for its two device-specific helpers: the
-    current-stream getter returns NULL and the "is a CUDA tensor" check asks for a CPU tensor.  The kernel objects of
+    Bayesian layers) and, when `sources` holds their kernels, of csrc/host_tokens.cpp (the token-model operators) over the CPU
+    model.  The sources are used as they are except for their device-specific helpers: the current-stream getter returns
+    NULL, no stream is being captured, and the "is a CUDA tensor" check asks for a CPU tensor.  The kernel objects of
     build(sources) are linked INTO the module (-Bsymbolic), so its C-ABI calls cannot bind to a libbde_hip.so the process
     may also hold."""
     import sysconfig
@@ -134,35 +156,32 @@ def build_host_nodes(sources):
     from torch.utils import cpp_extension as ce
     lib = build(sources)
     out_dir = os.path.dirname(lib)
-    text = open(os.path.join(CSRC, "host_autograd.cpp")).read()
-    old_stream = "void* current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }"
-    assert old_stream in text and "t.is_cuda() &&" in text and "#include <c10/hip/HIPStream.h>\n" in text
-    text = text.replace(old_stream, "void* current_stream(const at::Tensor&) { return nullptr; }")
-    old_capture = next(ln for ln in text.splitlines() if ln.startswith("bool stream_capturing(void* stream)"))
-    text = text.replace(old_capture, "bool stream_capturing(void*) { return false; }")
-    text = text.replace("t.is_cuda() &&", "!t.is_cuda() &&").replace("#include <c10/hip/HIPStream.h>\n", "")
-    text = text.replace('#include "../../include/bde_hip.h"', f'#include "{os.path.join(ROOT, "include", "bde_hip.h")}"')
-    text += "\nPYBIND11_MODULE(_bde_host_emu, m) { bind_autograd_nodes(m); }\n"
-    key = hashlib.sha256((text + torch.__version__).encode()).hexdigest()[:16]
+    texts = {n: _host_source(n) for n in ["host_autograd.cpp"] + (["host_tokens.cpp"] if TOKEN_SOURCES <= set(sources) else [])}
+    binds = ["bind_autograd_nodes"] + (["bind_token_nodes"] if len(texts) > 1 else [])
+    texts["host_autograd.cpp"] += "\nvoid bind_token_nodes(py::module_& m);\nPYBIND11_MODULE(_bde_host_emu, m) { " + \
+        " ".join(f"{b}(m);" for b in binds) + " }\n"
+    key = hashlib.sha256(("\0".join(texts.values()) + torch.__version__).encode()).hexdigest()[:16]
     out = os.path.join(out_dir, f"_bde_host_emu_{key}.so")
     if os.path.exists(out):
         return out
     with _locked():
         if os.path.exists(out):
             return out
-        return _build_host_nodes_locked(sources, text, out_dir, out)
+        return _build_host_nodes_locked(sources, texts, out_dir, out)
 
 
-def _build_host_nodes_locked(sources, text, out_dir, out):
+def _build_host_nodes_locked(sources, texts, out_dir, out):
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce
-    src = os.path.join(out_dir, "host_autograd_emu.cpp")
-    with open(src, "w") as fh:
-        fh.write(text)
+    srcs = []
+    for n, text in texts.items():
+        srcs.append(os.path.join(out_dir, n.replace(".cpp", "_emu.cpp")))
+        with open(srcs[-1], "w") as fh:
+            fh.write(text)
     objs = [os.path.join(out_dir, n.replace(".hip", ".cpp") + ".o") for n in sources] + [os.path.join(out_dir, "hip_emu.cpp.o")]
     libs = ce.library_paths()
-    cmd = ["g++", "-O1", "-std=c++17", "-shared", "-fPIC", src] + objs + ["-o", out + ".tmp", "-I" + sysconfig.get_paths()["include"],
+    cmd = ["g++", "-O1", "-std=c++17", "-shared", "-fPIC"] + srcs + objs + ["-o", out + ".tmp", "-I" + sysconfig.get_paths()["include"],
            "-DTORCH_EXTENSION_NAME=_bde_host_emu", "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-Wl,-Bsymbolic"]
     cmd += ["-I" + i for i in ce.include_paths()] + ["-L" + l for l in libs]
