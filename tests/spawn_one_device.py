@@ -2,13 +2,15 @@
 
 Several processes sharing a device can, rarely, lose a process to the HIP runtime's queue abort
 ``HSA_STATUS_ERROR_ILLEGAL_INSTRUCTION`` (SIGABRT) -- seen since round 2 with 8 ranks on one device, at a rate of about
-one run in 25-45 even with every code object of libbde_hip.so loaded up front (bde_init()).  DESIGN.md section 6 has the
-evidence and what round 4's fault hunt (tools/fault_hunt.sh) found.  The harness re-runs the ranks ONCE when EXACTLY that
-happens -- a rank died with SIGABRT *and* the ranks' stderr carries the runtime's HSA_STATUS_ERROR_ILLEGAL_INSTRUCTION
-queue-abort line -- records the event (``RETRIES`` here, ``gpurun_out/one_device_retries.log`` when that directory
-exists, and pytest's terminal summary through tests/conftest.py), and a SECOND such event in one pytest session fails
-the test.  Any other SIGABRT (a collective watchdog, a C++ assertion, a HIP launch failure), a Python exception in a
-rank, a wrong result: the test fails as usual.
+one run in 25-45 even with every code object of libbde_hip.so loaded up front (bde_init()); profiles/r04_fault_hunt.txt
+and profiles/r03_illegal_instruction_with_bde_init.txt hold what is known.  Ranks that use a device are NEVER started
+again after it: their test fails (``GPU_TEST``, set per test by tests/conftest.py; without it, wherever a device is
+visible).  Ranks that use none -- the harness's own tests -- are re-run ONCE when EXACTLY that happens -- a rank died with
+SIGABRT *and* the ranks' stderr carries the runtime's HSA_STATUS_ERROR_ILLEGAL_INSTRUCTION queue-abort line --, the event is
+recorded (``RETRIES`` here, ``gpurun_out/one_device_retries.log`` when that directory exists, and pytest's terminal
+summary through tests/conftest.py), and a SECOND such event in one pytest session fails the test.  Any other SIGABRT (a
+collective watchdog, a C++ assertion, a HIP launch failure), a Python exception in a rank, a wrong result: the test fails
+as usual.
 """
 import os
 import sys
@@ -16,11 +18,13 @@ import tempfile
 import time
 import warnings
 
+import torch
 import torch.multiprocessing as mp
 from torch.multiprocessing.spawn import ProcessExitedException
 
 FAULT_TEXT = "HSA_STATUS_ERROR_ILLEGAL_INSTRUCTION"
 MAX_RETRIES_PER_SESSION = 1
+GPU_TEST = None         # does the running test use a device? (tests/conftest.py; None: not known)
 RETRIES = []            # one entry per retried spawn of this pytest session: (time, nprocs, the runtime's abort line)
 
 
@@ -58,6 +62,9 @@ def spawn_ranks(fn, make_args, nprocs):
         and FAULT_TEXT in text
     if not is_fault:
         raise exc
+    on_device = torch.cuda.device_count() > 0 if GPU_TEST is None else GPU_TEST
+    if on_device:
+        raise RuntimeError(f"a rank died with SIGABRT and the runtime reported {FAULT_TEXT}; ranks on a device are not started again") from exc
     line = next((ln for ln in text.splitlines() if FAULT_TEXT in ln), "")[:300]
     RETRIES.append((time.strftime("%Y-%m-%d %H:%M:%S"), nprocs, line))
     out_dir = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gpurun_out")

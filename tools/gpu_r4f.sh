@@ -8,7 +8,6 @@ timeout 300 python tools/swag_batched_ab.py >> $O/swag_batched_rounds_ab.txt 2>&
 timeout 300 python tools/swag_batched_ab.py tools/bin/libbde_philox10.so >> $O/swag_batched_rounds_ab.txt 2>&1
 done
 grep -v amdgpu.ids $O/swag_batched_rounds_ab.txt
-bash tools/fault_hunt.sh 12 240 lazylog > $O/fault_hunt_lazylog.txt 2>&1; tail -60 $O/fault_hunt_lazylog.txt | cut -c1-240
 cd /tmp && export TMPDIR=/tmp && cd - > /dev/null
 timeout 900 rocprofv3 --kernel-trace --stats --output-format csv -d $O/prof -- python3 bench.py --gpus 1 --steps 20 --warmup 3 --no-cpu-baseline --no-config-extras > $O/bench_under_rocprof.json 2> $O/bench_under_rocprof.err
 find $O/prof -name "*kernel_stats.csv" | head -1 | xargs -I{} cp {} $O/kernel_stats.csv; head -30 $O/kernel_stats.csv | cut -c1-200
