@@ -16,7 +16,8 @@ using torch::autograd::variable_list;
 
 void* current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-bool stream_capturing(void* stream) { hipStreamCaptureStatus s = hipStreamCaptureStatusNone; return hipStreamIsCapturing(static_cast<hipStream_t>(stream), &s) == hipSuccess && s != hipStreamCaptureStatusNone; }
+// the capture a stream takes part in (0: none): one number per capture of the process
+uint64_t capture_of(void* stream) { hipStreamCaptureStatus s = hipStreamCaptureStatusNone; unsigned long long id = 0; return hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &s, &id) == hipSuccess && s != hipStreamCaptureStatusNone ? id + 1 : 0; }
 
 // the kernels produce plain tensors: a second differentiation through a node would silently see constants
 void check_once_differentiable(const variable_list& grad_outputs) {
@@ -180,7 +181,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_logits(const at::Tensor& log
 
 // Under sum / mean the forward writes the gradient for d objective / d loss = 1 in the pass that computes the loss; the backward
 // returns that buffer after a launch that leaves it alone where the value IS 1 and recomputes it from the logits where it is not.
-// Later backward passes of a retained graph, and one captured into a graph its forward is not part of, use a buffer of their own.
+// Later backward passes of a retained graph, and one that is not part of the very capture its forward was part of (captured
+// alone, or into another graph: replayed without that forward), use a buffer of their own.
 struct DistillNode : public torch::autograd::Function<DistillNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& values, const at::Tensor& indices,
                             const c10::optional<at::Tensor>& rest_, const c10::optional<at::Tensor>& weight_, int64_t reduction, double scale,
@@ -203,7 +205,7 @@ struct DistillNode : public torch::autograd::Function<DistillNode> {
                                    static_cast<int>(k), fdata(rows), fdata(loss), data(grad), fdata(inv), stream);
     if (rc != 0) refuse("bde_distill_fwd failed with code ", rc, rc == -1 ? " (invalid argument)" : " (hipError)");
     ctx->save_for_backward({logits, values, indices, rest, weight, inv});
-    ctx->saved_data["i"] = std::vector<int64_t>{reduction, stream_capturing(stream)};
+    ctx->saved_data["i"] = std::vector<int64_t>{reduction, static_cast<int64_t>(capture_of(stream))};
     ctx->saved_data["f"] = std::vector<double>{scale, temperature};
     if (grad.defined()) ctx->saved_data["unit"] = grad;
     return reduction == 0 ? rows : loss;
@@ -229,7 +231,7 @@ struct DistillNode : public torch::autograd::Function<DistillNode> {
         ctx->saved_data.erase(it);
       }
     }
-    const bool ready = grad.defined() && (i[1] != 0) == stream_capturing(stream);
+    const bool ready = grad.defined() && i[1] == static_cast<int64_t>(capture_of(stream));
     if (!ready) grad = at::empty({n, v}, z.options());
     const at::Tensor up = grad_outputs[0].contiguous();
     const int rc = bde_distill_bwd(data(z), type_code(z.scalar_type()), row_step(z), data(values), type_code(values.scalar_type()), data(indices),

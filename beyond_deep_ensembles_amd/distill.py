@@ -71,8 +71,8 @@ def _capturing(t) -> bool:
 class _Distill(torch.autograd.Function):
     """Under ``sum`` / ``mean`` the forward writes the gradient for d objective / d loss = 1 in the pass that computes the loss;
     the backward returns that buffer after a launch that leaves it alone where the value IS 1 and recomputes it from the logits
-    where it is not (one rounding either way).  Later backward passes of a retained graph, and one captured into a graph its
-    forward is not part of, compute into a buffer of their own."""
+    where it is not (one rounding either way).  Later backward passes of a retained graph, and passes that are captured -- a
+    graph may be replayed without the one that holds the forward --, compute into a buffer of their own."""
 
     @staticmethod
     def forward(ctx, logits, values, indices, rest, weight, reduction, scale, temperature, ops):
@@ -82,14 +82,14 @@ class _Distill(torch.autograd.Function):
         loss = inv = grad = None
         if reduction != "none":
             loss = torch.empty((), dtype=torch.float32, device=z.device)
-            if ctx.needs_input_grad[0]:
+            if ctx.needs_input_grad[0] and not _capturing(z):
                 grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         if reduction == "mean" and weight is not None:
             inv = torch.empty((), dtype=torch.float32, device=z.device)
         ops.distill_fwd(z, values, indices, rest, weight, loss_rows, loss=loss, grad=grad, inv_weight=inv, reduction=reduction, scale=scale,
                         temperature=temperature)
         ctx.save_for_backward(logits, values, indices, rest, weight, inv)
-        ctx.meta = (reduction, scale, temperature, ops, _capturing(z))
+        ctx.meta = (reduction, scale, temperature, ops)
         ctx.unit_grad = grad
         return loss_rows if reduction == "none" else loss
 
@@ -97,10 +97,10 @@ class _Distill(torch.autograd.Function):
     @once_differentiable          # the kernels produce plain tensors: no double backward
     def backward(ctx, g):
         logits, values, indices, rest, weight, inv = ctx.saved_tensors
-        reduction, scale, temperature, ops, captured = ctx.meta
+        reduction, scale, temperature, ops = ctx.meta
         z = logits.detach()
         grad, ctx.unit_grad = ctx.unit_grad, None
-        ready = grad is not None and captured == _capturing(z)
+        ready = grad is not None and not _capturing(z)
         if not ready:
             grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         ops.distill_bwd(z, values, indices, rest, weight, _dense(g, g.shape), grad, inv_weight=inv, mean=reduction == "mean", skip_if_one=ready,

@@ -138,8 +138,8 @@ def _host_source(name):
         assert line + "\n" in text, (name, line)
         text = text.replace(line, instead)
     if name == "host_tokens.cpp":
-        line = next(ln for ln in text.splitlines() if ln.startswith("bool stream_capturing(void* stream)"))
-        text = text.replace(line, "bool stream_capturing(void*) { return false; }")
+        line = next(ln for ln in text.splitlines() if ln.startswith("uint64_t capture_of(void* stream)"))
+        text = text.replace(line, "uint64_t capture_of(void*) { return 0; }")
     text = text.replace("t.is_cuda() &&", "!t.is_cuda() &&")
     return text.replace('#include "../../include/bde_hip.h"', f'#include "{os.path.join(ROOT, "include", "bde_hip.h")}"')
 
