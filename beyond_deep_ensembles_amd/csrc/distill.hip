@@ -10,8 +10,9 @@
 // i.e. the KL divergence between two distributions over K + 1 outcomes, the last one being "any other class".
 //
 // Numerics: everything fp32; the row is held in its own type and each gradient is rounded to that type once.  The listed
-// classes are masked out of the row before anything is summed, so Q is a sum of positive terms relative to the largest of
-// ITS terms (no 1 - sum cancellation, no underflow when the student puts nearly everything on the list).
+// classes are masked out of the row before anything is summed, so Q is a sum of positive terms (no 1 - sum cancellation).  Each
+// wave sums its part relative to a number near that part's largest element -- of its first granules, or, where the part rises far
+// above those, of all --, so nothing underflows when the student puts nearly everything on the list.
 #include "token_common.hpp"
 
 namespace bde {
@@ -280,13 +281,19 @@ __global__ __launch_bounds__(NT * kRowsPerGroup<NT>) void distill_topk_kernel(Di
   auto log_p = [&](int j) { return (t_l[j] - t_ref) * a.inv_tau - t_log; };
 
   if (a.loss && wave == 2 % W) {
+    // p (log p - log q), log q = gap / tau + inner - s_log.  A finite gap of 1e38 (a masked class) over a temperature below 1 may leave the range where
+    // the term does not: then p goes in first, and nothing else of the term counts beside it
+    auto term = [&](float p, float lp, float gap, float inner) {
+      const float x = gap * a.inv_tau;
+      return x == neg_inf() && gap > neg_inf() ? -(p * gap) * a.inv_tau : p * (lp - (x + inner - s_log));
+    };
     float acc = 0.0f;
     for (int j = lane; j < a.K; j += 64) {
       const float lp = log_p(j), p = exp2_hw(lp * kLog2e);
-      if (p != 0.0f) acc += p * (lp - ((z_l[j] - top) * a.inv_tau - s_log));
+      if (p != 0.0f) acc += term(p, lp, z_l[j] - top, 0.0f);
     }
     acc = wave_all_sum(acc);
-    if (r != 0.0f) acc += r * (r_log - ((other - top) * a.inv_tau + kLn2 * __builtin_amdgcn_logf(tail) - s_log));
+    if (r != 0.0f) acc += term(r, r_log, other - top, kLn2 * __builtin_amdgcn_logf(tail));
     if (lane == 0) a.loss[row] = silent ? 0.0f : factor * acc;
   }
   if constexpr (GRAD) {

@@ -89,3 +89,130 @@ def test_two_steps_captured_into_graphs_of_their_own():
             (gy,) = torch.autograd.grad(want, y)
             assert torch.equal(outs[i][0], want) and torch.equal(outs[i][1], gy)
             outs[i][1].zero_()
+
+
+# ---- masks of the type's lowest value, temperatures below 1: against a reference that subtracts the row's maximum before it
+# divides by the temperature (numbers of 3e38 lose everything else otherwise), with tolerances that no mask widens
+def log_shares(x, tau, dim=1):
+    """log softmax(x / tau) in 64 bits; -inf where x is -inf, and rows of -inf alone are -inf."""
+    x = x.double()
+    top = x.amax(dim, keepdim=True)
+    y = (x - torch.where(top == -math.inf, 0.0, top)) / tau
+    return y - torch.log(torch.exp(y).sum(dim, keepdim=True))
+
+
+def masked_distill64(z, values, indices, rest, tau):
+    """Losses of the rows, d loss / d z and, per row, the largest difference of exponents that a share above 2^-126 comes from."""
+    n, v = z.shape
+    # the teacher in units of the temperature, relative to its largest entry (rest already is in those units)
+    t = values.double()
+    top = t.amax(1, keepdim=True)
+    r = torch.full((n, 1), -math.inf, dtype=torch.float64) if rest is None else rest.double()[:, None] - top / tau
+    t = torch.cat([(t - top) / tau, r], 1)
+    t = t - t.amax(1, keepdim=True)
+    lp = t - torch.log(torch.exp(t).sum(1, keepdim=True))
+    p = lp.exp()
+    listed = torch.zeros(n, v, dtype=torch.bool).scatter_(1, indices, True)
+    lq = log_shares(z, tau)
+    inside = log_shares(z.masked_fill(listed, -math.inf), tau)              # shares among the others alone
+    zd = z.double()
+    others = zd.masked_fill(listed, -math.inf)
+    o_top, top = others.amax(1, keepdim=True), zd.amax(1, keepdim=True)
+    l_tail = (o_top - top) / tau + torch.log(torch.exp((others - o_top) / tau).sum(1, keepdim=True)) - torch.log(torch.exp((zd - top) / tau).sum(1, keepdim=True))
+    both = torch.cat([lq.gather(1, indices), l_tail], 1)
+    terms = torch.where(p > 2.0 ** -126, p * (lp - both), 0.0)
+    q = lq.exp()
+    spread_p = torch.zeros(n, v, dtype=torch.float64).scatter_add_(1, indices, p[:, :-1])
+    other = torch.where(p[:, -1:] > 0, p[:, -1:] * inside.exp(), 0.0)
+    grad = torch.where(listed, q - spread_p, q - other) / tau
+    size = torch.where(listed, q + spread_p, q + other) / tau
+
+    def reach(x, share):
+        return torch.where(share > 2.0 ** -126, (x - x.amax(1, keepdim=True)).abs() / tau, 0.0).amax(1)
+    spread = reach(zd, q) + reach(others, inside.exp()) + reach(values.double(), p[:, :-1])
+    return terms.sum(1), terms.abs().sum(1), grad, size, spread
+
+
+def check_masked(backend, z, values, indices, rest, tau):
+    ops, dev = backend
+    put = lambda t: None if t is None else t.to(dev)                    # noqa: E731
+    x = z.to(dev).requires_grad_()
+    rows = bde.distillation_loss(x, put(values), put(indices), put(rest), temperature=tau, reduction="none", _ops=ops)
+    (got,) = torch.autograd.grad(rows, x, torch.ones_like(rows))
+    want, size, grad, gsize, spread = masked_distill64(z, values, indices, rest, tau)
+    # exponents: log2(e) / tau three roundings off, a difference and a product one each, relative to the spread of what has a
+    # share; exp and log one step (2 u) each and ln 2 one; sums of v <= 64 and K <= 8 terms; the products of a term and their sum
+    rel = (5 * spread + 2 * 64 + 40) * U
+    rows = rows.detach().cpu().double()
+    # where a masked class has a share p, the term is p (relative error rel, as everywhere) times a difference of exponents of
+    # 1e38: one rounding for that difference, two for the temperature (its inverse, the product), one for the product with p and
+    # three for its place in the sum -- relative to the term, so 8 u of the sizes' sum beside rel
+    off = (rows - want).abs()
+    bound = rel * (size + 2) + 8 * U * size
+    assert torch.isfinite(want).all() and (off <= bound).all(), f"losses {rows.tolist()}, expected {want.tolist()}"
+    off = (got.cpu().double() - grad).abs() - (gsize * (rel + 6 * U)[:, None] + grad.abs() * U + 2.0 ** -125)
+    assert off.max().item() <= 0, f"gradient {off.max().item():.3e} beyond the tolerance"
+
+
+LOWEST = torch.finfo(F32).min
+
+
+@pytest.mark.parametrize("tau", [0.5, 0.6, 1.0, 2.0])
+@pytest.mark.parametrize("what", ["some_others", "others", "a_listed", "all", "teacher", "teacher_and_others", "teacher_entry"])
+def test_distill_masked_with_the_lowest_value(backend, what, tau):
+    """Classes the student masks, classes the teacher masks, and a teacher whose whole list is masked (uniform over the list where
+    nothing is left beside it).  Masked classes that the teacher gives something make losses of 1e35 and more: finite as long as
+    they fit."""
+    z, values, indices, rest = teacher(6, 30, 5, F32, 11, tau)
+    # little is left beside the list, so that a loss of the others' masks fits fp32 at every temperature here
+    rest = torch.logsumexp(values.double() / tau, 1).float() - 6.0
+    listed = torch.zeros(6, 30, dtype=torch.bool).scatter_(1, indices, True)
+    if what == "some_others":
+        z = z.masked_fill(~listed & (torch.arange(30) % 3 == 0), LOWEST)
+    elif what == "others":
+        z = z.masked_fill(~listed, LOWEST)
+    elif what == "a_listed":
+        values[:, 2] = values.amin(1) - 8.0 * tau                       # the masked class has a small share
+        z.scatter_(1, indices[:, 2:3], LOWEST)
+    elif what == "all":
+        z = torch.full_like(z, LOWEST)
+    elif what == "teacher_entry":
+        values[:, 1:3] = LOWEST
+    else:
+        values = torch.full_like(values, LOWEST)
+        rest = torch.full_like(rest, -math.inf)
+        if what == "teacher_and_others":
+            z = z.masked_fill(~listed, LOWEST)
+    check_masked(backend, z, values, indices, rest, tau)
+
+
+@pytest.mark.parametrize("tau", [0.5, 1.0])
+def test_the_masked_reference_notices_small_mistakes(tau):
+    """The oracle's tolerances are those of the kernel, not of the mask: a loss off by 1%, a uniform teacher's share of 1."""
+    z, values, indices, rest = teacher(6, 30, 5, F32, 11, tau)
+    values, rest = torch.full_like(values, LOWEST), torch.full_like(rest, -math.inf)
+    want, size, grad, gsize, spread = masked_distill64(z, values, indices, rest, tau)
+    rel = (5 * spread + 2 * 64 + 40) * U
+    assert (0.01 * want.abs() > rel * (size + 2)).all()
+    p = torch.full((6, 5), 0.2, dtype=torch.float64)
+    # the same loss by hand: five classes of a fifth each against the student's log-shares
+    lq = log_shares(z, tau).gather(1, indices)
+    assert torch.allclose((p * (math.log(0.2) - lq)).sum(1), want, rtol=0, atol=1e-12)
+    assert (0.8 / tau > 1000 * (gsize * rel[:, None]).max()).all()
+
+
+@pytest.mark.parametrize("tau", [0.5, 1.0])
+@pytest.mark.parametrize("v,k", [(50, 7), (3001, 20)])
+def test_topk_rest_of_rows_masked_with_the_lowest_value(backend, v, k, tau):
+    """The masked classes add nothing to the rest, and widen no tolerance."""
+    ops, dev = backend
+    z = torch.randn(2, v, generator=gen(v))
+    z = z.masked_fill(torch.rand(2, v, generator=gen(v + 1)) < 0.5, LOWEST)
+    got = bde.topk_logits(z.to(dev), k, temperature=tau, _ops=ops)
+    order = torch.sort(z.double(), dim=1, descending=True, stable=True)
+    assert torch.equal(got.indices.cpu(), order.indices[:, :k]) and torch.equal(got.values.cpu().double(), order.values[:, :k])
+    left = order.values[:, k:]
+    top = left[:, :1]
+    want = top[:, 0] / tau + torch.log(torch.exp((left - top) / tau).sum(1))
+    spread = 2 * 8.0 / tau                             # (the normal numbers here lie within 4 of 0)
+    assert ((got.rest.cpu().double() - want).abs() <= U * (56 + v / 8192 + 8 * spread) + 4 * U * want.abs()).all()
