@@ -42,9 +42,10 @@ struct EmbedArgs {
   int piece;
   int log_groups, bucket;  // workgroups of the sort (a power of two) and the most tokens one of them owns
   int chunk;               // > 0: the tokens are dealt out to the sort's workgroups first, this many per workgroup of that
-  int* counts;             // [chunks][groups]
-  int* group_start;        // [groups + 1]
-  int* dealt_p;            // [N] positions by group, in order
+  int log_deal;            // into a power of two of groups, each for one workgroup of the sort or for several
+  int* counts;             // [chunks][dealt groups]
+  int* group_start;        // [dealt groups + 1]
+  int* dealt_p;            // [N] positions by dealt group, in order
   int* dealt_t;            // [N] their tokens
   int stream_zeros;        // zero rows are stored past the caches
   int join0;               // first workgroup of this launch of the join
@@ -154,7 +155,10 @@ __device__ __forceinline__ bool live_token(const EmbedArgs& a, int64_t raw) {   
 
 // With many tokens the workgroups do not read all of them: two short kernels deal the positions out first (count per chunk and
 // group; then each chunk writes its positions behind those of the chunks before it).  Gradient of a 30,011 x 256
-// fp32 table: 32,768 tokens 35 us without, 39 with; 65,536 tokens 65 and 49; 262,144 tokens 202 and 118.
+// fp32 table: 32,768 tokens 35 us without, 39 with; 65,536 tokens 65 and 49; 262,144 tokens 202 and 118.  A large table takes more
+// workgroups in the sort than are dealt to (kMaxDealGroups): token t goes to group t mod that number, and the workgroups b, b +
+// that number, ... of the sort read the group's share and find their own in it (when all of them read all tokens: 262,208 x 64, 65,536
+// tokens 85 us against 64; 1,048,576 x 64, 262,144 tokens 386 against 147).
 __global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(EmbedArgs a, int log_groups) {
   __shared__ int count[kMaxDealGroups];
   const int groups = 1 << log_groups, n = static_cast<int>(a.N);
@@ -286,7 +290,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
   for (int i = tid; i < kSortWaves * a.bucket; i += kSortThreads) hist[i] = 0;
   __syncthreads();
   int* const mine = hist + wave * a.bucket;
-  const int first = DEALT ? a.group_start[group] : 0, n = DEALT ? a.group_start[group + 1] : static_cast<int>(a.N);
+  const int deal = DEALT ? group & ((1 << a.log_deal) - 1) : 0;
+  const int first = DEALT ? a.group_start[deal] : 0, n = DEALT ? a.group_start[deal + 1] : static_cast<int>(a.N);
   const int chunk = ((n - first + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int begin = min(n, first + wave * chunk), end = min(n, begin + chunk);
   const unsigned long long before = (1ull << lane) - 1ull;
@@ -352,14 +357,10 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
   if (tid < own) totals[tid] = total;
   int all;
   int start = first + scan_threads(total, sums, &all);
-  if constexpr (!DEALT) {
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      start += below[w];
-      all += below[w];
-    }
-  } else {
-    all += first;
+  for (int w = 0; w < kSortWaves; ++w) {
+    start += below[w];
+    all += below[w];
   }
   if (tid < own) {
     for (int w = 0; w < kSortWaves; ++w) {
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(EmbedArgs 
       start += c;
     }
   }
-  if (tid == 0 && group == groups - 1) a.header[0] = all;
+  if (tid == 0 && group == groups - 1) a.header[0] = DEALT ? a.group_start[1 << a.log_deal] : all;
   __syncthreads();
   // positions in order: lanes of one token take consecutive places
   const int bits = 32 - __builtin_clz(a.bucket | 1);
@@ -732,9 +733,9 @@ static int embedding_bwd_launch(EmbedArgs a, hipStream_t s) {
   const size_t lds = sizeof(int) * kSortWaves * a.bucket;
   if (a.chunk > 0) {
     const int chunks = static_cast<int>((a.N + a.chunk - 1) / a.chunk);
-    hipLaunchKernelGGL(embedding_count_kernel, dim3(chunks), dim3(kSortThreads), 0, s, a, a.log_groups);
+    hipLaunchKernelGGL(embedding_count_kernel, dim3(chunks), dim3(kSortThreads), 0, s, a, a.log_deal);
     if (const int rc = to_err(hipGetLastError())) return rc;
-    hipLaunchKernelGGL(embedding_deal_kernel, dim3(chunks), dim3(kSortThreads), 0, s, a, a.log_groups, chunks);
+    hipLaunchKernelGGL(embedding_deal_kernel, dim3(chunks), dim3(kSortThreads), 0, s, a, a.log_deal, chunks);
     if (const int rc = to_err(hipGetLastError())) return rc;
     hipLaunchKernelGGL((embedding_sort_kernel<TW, true>), groups, dim3(kSortThreads), lds, s, a, a.log_groups);
   } else {
@@ -848,7 +849,8 @@ extern "C" int bde_embedding_bwd(const void* g, int g_dtype, int64_t ldg, const 
   a.bucket = static_cast<int>((V + (1 << a.log_groups) - 1) >> a.log_groups);
   char* rest = base + 256 + 2 * list;
   if (embedding_chunk(N) > 0) {
-    if ((1 << a.log_groups) <= kMaxDealGroups) a.chunk = embedding_chunk(N);
+    a.chunk = embedding_chunk(N);
+    while (a.log_deal < a.log_groups && (2 << a.log_deal) <= kMaxDealGroups) ++a.log_deal;
     a.counts = reinterpret_cast<int*>(rest);
     a.group_start = a.counts + 256 * kMaxDealGroups;
     a.dealt_p = reinterpret_cast<int*>(rest + kDealBytes);

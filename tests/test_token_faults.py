@@ -216,3 +216,70 @@ def test_topk_rest_of_rows_masked_with_the_lowest_value(backend, v, k, tau):
     want = top[:, 0] / tau + torch.log(torch.exp((left - top) / tau).sum(1))
     spread = 2 * 8.0 / tau                             # (the normal numbers here lie within 4 of 0)
     assert ((got.rest.cpu().double() - want).abs() <= U * (56 + v / 8192 + 8 * spread) + 4 * U * want.abs()).all()
+
+
+# ---- the gradient of large tables (the kernels alone: no autograd node lies between)
+@pytest.fixture(params=["emu", pytest.param("hip", marks=pytest.mark.gpu)])
+def kernels(request):
+    if request.param == "emu":
+        from tests.hip_emu import build, emu_ops
+        if not build.available():
+            pytest.skip("no host clang / HIP headers to build the CPU model with")
+        with emu_ops.emulated(emu_ops.ALL) as ops:
+            yield ops, torch.device("cpu")
+        return
+    from beyond_deep_ensembles_amd.ops import HipOps
+    yield HipOps(), torch.device("cuda:0")
+
+
+def check_table_gradient(kernels, n, v, d, dtype, seed, pad):
+    """The lookup's gradient over a table of many rows against float64 sums of the touched rows; all other rows are zero."""
+    ops, dev = kernels
+    g = gen(seed)
+    tokens = (v * torch.rand(n, generator=g, dtype=torch.float64) ** 3).long()
+    tokens[:4] = torch.tensor([v - 1, 0, -1, v])                        # the ends, and two outside
+    tokens[n // 2:n // 2 + n // 8] = v - 2                              # a run of its own
+    grad = torch.randn(n, d, generator=g).to(dtype)
+    got = torch.full((v, d), 7.0, device=dev)
+    ops.embedding_bwd(grad.to(dev), tokens.to(dev), got, scale=0.5, padding_idx=pad)
+    if dev.type != "cpu":
+        again = torch.full((v, d), 7.0, device=dev)
+        ops.embedding_bwd(grad.to(dev), tokens.to(dev), again, scale=0.5, padding_idx=pad)
+        assert torch.equal(got, again)
+    live = (tokens >= 0) & (tokens < v) & (tokens != pad)
+    rows, place = torch.unique(tokens[live], return_inverse=True)
+    want = torch.zeros(len(rows), d, dtype=torch.float64).index_add_(0, place, grad[live].double()) * 0.5
+    size = torch.zeros(len(rows), d, dtype=torch.float64).index_add_(0, place, grad[live].double().abs()) * 0.5
+    count = torch.bincount(place, minlength=len(rows)).double()[:, None]
+    # count terms added one by one (parts of a sum only shorten the chain), the scale exact
+    assert ((got.cpu()[rows].double() - want).abs() <= size * (count + 1) * U * 1.01).all()
+    got[rows.to(dev)] = 0.0
+    assert int(torch.count_nonzero(got)) == 0
+
+
+@pytest.mark.parametrize("n,v,d,dtype", [(700, 131073, 2, F32), (600, 262145, 1, BF16), (600, 262208, 3, F32), (49200, 262208, 1, BF16),
+                                         (49999, 530001, 1, F32)])
+def test_embedding_gradient_of_large_tables(kernels, n, v, d, dtype):
+    """Several launches over more workgroups than the device has at once; many tokens over more groups than they are dealt out
+    to."""
+    if kernels[1].type == "cpu" and (n, v) not in ((700, 131073), (600, 262208)):
+        pytest.skip("on the CPU model two of the five (a minute each), and the dealt case below")
+    check_table_gradient(kernels, n, v, d, dtype, n + v, pad=3)
+
+
+def test_tokens_of_large_tables_are_not_read_by_every_workgroup(kernels):
+    """With many tokens each workgroup of the sort reads its share of them, whatever the table's size: the work is not tokens
+    times rows (counted on the CPU model)."""
+    ops, dev = kernels
+    if dev.type != "cpu":
+        pytest.skip("the CPU model counts the bytes")
+    from tests.hip_emu.emu_ops import Traffic
+    n, v = 49200, 300001
+    tokens = torch.randint(0, v, (n,), generator=gen(0))
+    grad, table = torch.ones(n, 1), torch.empty(v, 1)
+    with Traffic(ops) as t:
+        ops.embedding_bwd(grad, tokens, table)
+    assert t.of(tokens)[0] <= 4 * 8 * n                                 # counted, counted per wave, dealt out
+    assert torch.equal(table, torch.bincount(tokens, minlength=v).float()[:, None])
+    # nothing else is read in proportion to tokens x workgroups: the lists, the gradient and its parts come to a few words a token
+    assert t.read <= 400 * n + 64 * 4 * v
