@@ -560,11 +560,31 @@ class BBBEmbedding(_LocalReparamLayer):
                                   padding_idx=self.padding_idx, out_dtype=self.out_dtype, _ops=w._get_ops())
 
 
+def _plain_table(child) -> bool:
+    return isinstance(child, nn.Embedding) and child.max_norm is None and not child.scale_grad_by_freq and not child.sparse \
+        and child.weight.dtype == torch.float32
+
+
+def _refuse_shared_tables(module):
+    """A table with more than one place in the model: a Gaussian for each would untie them."""
+    places = {}
+    for name, p in module.named_parameters(remove_duplicate=False):
+        places.setdefault(id(p), []).append(name)
+    for child in module.modules():
+        if _plain_table(child) and len(places[id(child.weight)]) > 1:
+            raise ValueError(f"make_module_bbb: {', '.join(places[id(child.weight)])} share one parameter; replacing the embedding would give each "
+                             "a Gaussian of its own")
+
+
 def make_module_bbb(module: nn.Module, prior, *, embeddings: bool = False, **kwargs) -> int:
     """Replace every nn.Linear / nn.Conv2d of ``module`` by its mean-field counterpart, keeping the
     current weights as the means (cf. the reference's ``make_module_bbb``); returns the number of
-    layers replaced.  ``embeddings=True`` replaces its nn.Embedding tables (plain lookups: no ``max_norm``,
-    ``scale_grad_by_freq``, ``sparse``; a ScaledEmbedding keeps its scale) by BBBEmbedding as well."""
+    layers replaced.  ``embeddings=True`` replaces its nn.Embedding tables (float32 ones that look up and do nothing else: no
+    ``max_norm``, ``scale_grad_by_freq``, ``sparse``; others stay as they are; a ScaledEmbedding keeps its scale) by
+    BBBEmbedding as well.  A table that has more than one place in the model -- an output layer tied to it, two lookups -- is
+    refused before anything is replaced."""
+    if embeddings:
+        _refuse_shared_tables(module)
     replaced = 0
     for name, child in list(module.named_children()):
         new = None
@@ -574,8 +594,7 @@ def make_module_bbb(module: nn.Module, prior, *, embeddings: bool = False, **kwa
                 and child.kernel_size[0] == child.kernel_size[1] and isinstance(child.padding, tuple):
             new = BBBConv2d(child.in_channels, child.out_channels, child.kernel_size[0], prior, prior,
                             stride=child.stride, padding=child.padding, bias=child.bias is not None, **kwargs)
-        elif embeddings and isinstance(child, nn.Embedding) and child.max_norm is None and not child.scale_grad_by_freq \
-                and not child.sparse and child.weight.dtype == torch.float32:
+        elif embeddings and _plain_table(child):
             new = BBBEmbedding(child.num_embeddings, child.embedding_dim, prior, child.padding_idx, scale=getattr(child, "scale", 1.0),
                                out_dtype=getattr(child, "out_dtype", None), **kwargs)
         if new is not None:

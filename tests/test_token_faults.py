@@ -283,3 +283,43 @@ def test_tokens_of_large_tables_are_not_read_by_every_workgroup(kernels):
     assert torch.equal(table, torch.bincount(tokens, minlength=v).float()[:, None])
     # nothing else is read in proportion to tokens x workgroups: the lists, the gradient and its parts come to a few words a token
     assert t.read <= 400 * n + 64 * 4 * v
+
+
+# ---- replacing tables of a model
+class _Tied(torch.nn.Module):
+    """The output layer shares the input table."""
+
+    def __init__(self):
+        super().__init__()
+        self.body = torch.nn.Sequential(torch.nn.Embedding(9, 4), torch.nn.Linear(4, 4))
+        self.head = torch.nn.Linear(4, 9, bias=False)
+        self.head.weight = self.body[0].weight
+
+
+class _Shared(torch.nn.Module):
+    """Two parts of the model look up in one table."""
+
+    def __init__(self):
+        super().__init__()
+        self.encoder = torch.nn.Sequential(torch.nn.Embedding(9, 4), torch.nn.Linear(4, 4))
+        self.decoder = torch.nn.Sequential(self.encoder[0], torch.nn.Linear(4, 4))
+
+
+@pytest.mark.parametrize("model", [_Tied, _Shared])
+def test_make_module_bbb_refuses_to_untie_a_table(backend, model):
+    """Each place would get a Gaussian of its own; the model is left as it was."""
+    ops, dev = backend
+    net = model().to(dev)
+    before = [type(m) for m in net.modules()]
+    with pytest.raises(ValueError, match="share"):
+        bde.make_module_bbb(net, bde.GaussianPrior(0, 1.0), embeddings=True, _ops=ops)
+    assert [type(m) for m in net.modules()] == before
+
+
+def test_make_module_bbb_leaves_tables_it_does_not_take(backend):
+    """16-bit tables and lookups that do more than look up stay as they are."""
+    ops, dev = backend
+    net = torch.nn.ModuleList([torch.nn.Embedding(9, 4, dtype=BF16), torch.nn.Embedding(9, 4, max_norm=1.0),
+                               torch.nn.Embedding(9, 4, scale_grad_by_freq=True), torch.nn.Embedding(9, 4)]).to(dev)
+    assert bde.make_module_bbb(net, bde.GaussianPrior(0, 1.0), embeddings=True, _ops=ops) == 1
+    assert [type(m) is bde.BBBEmbedding for m in net] == [False, False, False, True]
