@@ -81,6 +81,15 @@ __global__ __launch_bounds__(kBlock) void svgd_fused_kernel(float* __restrict__ 
 #pragma unroll
         for (int c = 0; c < 4; ++c) u[i][c] = __builtin_fmaf(b, p[j][c], __builtin_fmaf(a, g[c], u[i][c]));
       }
+      // One particle's terms at a time.  Left to itself the compiler takes the columns' components one after the other (the SGD
+      // chain starts with the first), so all 2 M^2 coefficients are wanted four times over, do not fit the scalar registers and come
+      // back from parked lanes, an instruction per FMA: full steps of 23.9 M coordinates at M = 5 / 8 / 10 / 16 282 / 580 / 1,160 /
+      // 5,160 us against 271 / 439 / 600 / 922 (with the Gram, M = 8: 617 against 496).  Adam's form does not do that, and holding
+      // it to this order costs it: M = 8 451 against 497, M = 16 949 against 1,245.
+      if constexpr (OPT == 0) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) asm volatile("" : "+v"(u[i]));
+      }
     }
     // u[i] = -phi_i: the gradient the reference hands to the base optimizer (svgd.py:95)
     f32x4 a0, a1;
