@@ -23,7 +23,8 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "beyond_deep_ensembles_amd", "csrc")
 HIPCC = "/opt/rocm/bin/hipcc"
-FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-ffp-contract=off", "-fno-fast-math", "-I" + os.path.join(ROOT, "include"),
+FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-ffp-contract=off", "-fno-fast-math", "-Xclang", "-target-feature",
+         "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"),
          "--cuda-device-only", "-S"]
 # preferred instantiations (substrings of the demangled name): the BASELINE operating points
 PICK = {"svgd_combine_kernel": "<8, true>", "svgd_combine_seg_kernel": "<8>", "svgd_fused_kernel": "<8, 0, false, false>",

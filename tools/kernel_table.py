@@ -19,8 +19,8 @@ CSRC = os.path.join(ROOT, "beyond_deep_ensembles_amd", "csrc")
 BEGIN, END = "<!-- KERNEL-TABLE:BEGIN (tools/kernel_table.py --write) -->", "<!-- KERNEL-TABLE:END -->"
 
 # device status keys
-R3 = "yes -- green in the driver's r03 suite (GPUTEST_r03), source unchanged since"
-R4B = "yes -- green in builder calls r4b/r4c (profiles/r04_pytest_gpu_call_{b,c}.log) after its last change"
+R3 = "yes -- green in the driver's r03 suite and, compiled without packed fp32, in r07's (GPUTEST_r03, _r07)"
+R4B = "yes -- green in builder calls r4b/r4c (profiles/r04_pytest_gpu_call_{b,c}.log) and, compiled without packed fp32, in the r07 suite"
 TOK = "yes -- green with `tests/test_token_ops.py` (`-m gpu`)"
 NEVER = ("**no** -- changed after the last GPU call (pool closed since round 4); runs on the CPU model only; NOT a default path "
          "until `device_verified.json` records a green device run of these sources (§0)")
@@ -42,7 +42,7 @@ ROWS = {
     "svgd_gather_seg_kernel": ("packs segmented gradients into flat rows (collectives, small-model kernel, M > 16)", "`8·rows·D` B",
                                "6.0 TB/s (0.75); r3 `r03_seg_bench.txt`", R3, "`test_svgd_segmented_gradients_equal_flat_rows`"),
     "svgd_fused_kernel": ("`svgd.py:86-103` incl. the M `base_optimizer.step()` calls (SGD / Adam, shared state Q5) + next step's Gram",
-                          "`(12M+8)·D` (SGD) / `(12M+16)·D` (Adam) B", "0.4725 ms = 5.26 TB/s (0.657) full step, M=8; r4 bench line", R3,
+                          "`(12M+8)·D` (SGD) / `(12M+16)·D` (Adam) B", "0.500 ms = 4.97 TB/s (0.62) full step with the next step's Gram, 0.440 without, M=8 SGD; Adam 0.479 / 0.453; `svgd_fused_sgd_lane_reads.txt`", R3,
                           "`test_svgd_fused_optimizers_match_torch_shared_state`, `test_svgd_trajectory[hip-*]`"),
     "svgd_apply_sgd_kernel": ("the M shared-state SGD applications alone (`svgd.py:92-103`), 17 ≤ M ≤ 64", "`(12M+8)·D` B",
                               "0.995 ms step+apply (0.70); r4 bench line", R3, "`test_svgd_many_particles_one_apply_launch_equals_the_optimizer_loop`"),
@@ -65,7 +65,7 @@ ROWS = {
     "swag_sample_kernel": ("`swag.py:57,112-114`: `mean + W@eps_W + sqrt(diag)·eps_D`", "`4·D·(K+3)` B (+4D with supplied eps_D)",
                            "0.3666 ms = 5.99 TB/s (0.749), K=20; r4 bench line", R4B, "`test_swag_sample_golden_and_oracle`"),
     "swag_sample_batched_dma_kernel": ("S samples per pass, `[S,K]×[K,D]` on `v_mfma_f32_32x32x2_f32`, K ≤ 20, next tile via LDS-DMA", "`4·D·(K+2+S)` B",
-                                       "0.918–0.952 ms for S=30 = 5.2–5.4 TB/s (0.65–0.68); 0.995–1.003 of its R22 W30 probe `r04_swag_batched_vs_probe.txt`", R4B,
+                                       "0.918–0.952 ms for S=30 = 5.2–5.4 TB/s (0.65–0.68); 0.995–1.003 of its R22 W30 probe `r04_swag_batched_vs_probe.txt`; 1.00 ms (0.62) compiled without packed fp32", R4B,
                                        "`test_swag_batched_sampler_both_kernels_equal_single_samples`"),
     "swag_sample_batched_kernel": ("the same, register kernel (K > 20)", "`4·D·(K+2+S)` B", "0.712 of 8 TB/s at K=20 `r04_swag_batched_ab.txt`", R4B, "same test"),
     "philox_normal_kernel": ("noise hook (tests, small activations)", "`4·D` B", "—", R3, "`test_kernel_normals_equal_the_checker_transform`"),

@@ -1,6 +1,6 @@
 // Kernel experiment harness (development tool, not part of the product):
 // times kernel variants in ONE process with hipEvents (interleaved rounds).
-// build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -I include tools/kexp.hip -o gpurun_out/kexp
+// build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -I include tools/kexp.hip -o gpurun_out/kexp
 #include "../beyond_deep_ensembles_amd/csrc/svgd.hip"
 #include <cstdio>
 #include <vector>

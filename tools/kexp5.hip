@@ -3,7 +3,7 @@
 //      this device (the ceiling every streaming kernel of the library is compared with);
 //   2. partitioning / loads-in-flight variants of the sampling kernels (swag_sample, gauss_draw_fwd);
 //   3. Gram-pass variants; 4. small-model SVGD step: single launch vs three stages; 5. product kernels.
-// Build: hipcc -O3 --offload-arch=gfx950 tools/kexp5.hip -Lbeyond_deep_ensembles_amd/lib -lbde_hip ...
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/kexp5.hip -Lbeyond_deep_ensembles_amd/lib -lbde_hip ...
 #include "../beyond_deep_ensembles_amd/csrc/svgd_gram.hpp"
 #include <cstdio>
 #include <cstring>

@@ -1,5 +1,5 @@
 // Issue rate of v_mfma_f32_32x32x2_f32 on gfx950: N dependent-distance-4 products per wave, W waves per SIMD.
-//   hipcc -O3 --offload-arch=gfx950 tools/mfma_rate.hip -o tools/bin/mfma_rate && tools/bin/mfma_rate
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_rate.hip -o tools/bin/mfma_rate && tools/bin/mfma_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 using f32x16 = __attribute__((ext_vector_type(16))) float;
