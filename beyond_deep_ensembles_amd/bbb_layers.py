@@ -571,8 +571,9 @@ def _refuse_shared_tables(module):
     for name, p in module.named_parameters(remove_duplicate=False):
         places.setdefault(id(p), []).append(name)
     for child in module.modules():
-        if _plain_table(child) and len(places[id(child.weight)]) > 1:
-            raise ValueError(f"make_module_bbb: {', '.join(places[id(child.weight)])} share one parameter; replacing the embedding would give each "
+        names = places.get(id(child.weight), ()) if _plain_table(child) else ()
+        if len(names) > 1:
+            raise ValueError(f"make_module_bbb: {', '.join(names)} share one parameter; replacing the embedding would give each "
                              "a Gaussian of its own")
 
 

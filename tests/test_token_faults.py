@@ -323,3 +323,17 @@ def test_make_module_bbb_leaves_tables_it_does_not_take(backend):
                                torch.nn.Embedding(9, 4, scale_grad_by_freq=True), torch.nn.Embedding(9, 4)]).to(dev)
     assert bde.make_module_bbb(net, bde.GaussianPrior(0, 1.0), embeddings=True, _ops=ops) == 1
     assert [type(m) is bde.BBBEmbedding for m in net] == [False, False, False, True]
+
+
+def test_make_module_bbb_takes_a_table_whose_weight_is_computed(backend):
+    """A parametrised table's weight is no parameter of its own: it is in one place."""
+    ops, dev = backend
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2.0 * w
+    table = torch.nn.Embedding(9, 4)
+    torch.nn.utils.parametrize.register_parametrization(table, "weight", Twice())
+    net = torch.nn.Sequential(table).to(dev)
+    want = table.weight.detach().clone()
+    assert bde.make_module_bbb(net, bde.GaussianPrior(0, 1.0), embeddings=True, _ops=ops) == 1
+    assert torch.equal(net[0].weight.mean, want)
