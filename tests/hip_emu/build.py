@@ -150,7 +150,7 @@ def build_host_nodes(sources):
     model.  The sources are used as they are except for their device-specific helpers: the current-stream getter returns
     NULL, no stream is being captured, and the "is a CUDA tensor" check asks for a CPU tensor.  The kernel objects of
     build(sources) are linked INTO the module (-Bsymbolic), so its C-ABI calls cannot bind to a libbde_hip.so the process
-    may also hold."""
+    may also hold; every build's module has a name of its own (a process may load several)."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce
@@ -158,7 +158,7 @@ def build_host_nodes(sources):
     out_dir = os.path.dirname(lib)
     texts = {n: _host_source(n) for n in ["host_autograd.cpp"] + (["host_tokens.cpp"] if TOKEN_SOURCES <= set(sources) else [])}
     binds = ["bind_autograd_nodes"] + (["bind_token_nodes"] if len(texts) > 1 else [])
-    texts["host_autograd.cpp"] += "\nvoid bind_token_nodes(py::module_& m);\nPYBIND11_MODULE(_bde_host_emu, m) { " + \
+    texts["host_autograd.cpp"] += "\nvoid bind_token_nodes(py::module_& m);\nPYBIND11_MODULE(TORCH_EXTENSION_NAME, m) { " + \
         " ".join(f"{b}(m);" for b in binds) + " }\n"
     key = hashlib.sha256(("\0".join(texts.values()) + torch.__version__).encode()).hexdigest()[:16]
     out = os.path.join(out_dir, f"_bde_host_emu_{key}.so")
@@ -182,7 +182,7 @@ def _build_host_nodes_locked(sources, texts, out_dir, out):
     objs = [os.path.join(out_dir, n.replace(".hip", ".cpp") + ".o") for n in sources] + [os.path.join(out_dir, "hip_emu.cpp.o")]
     libs = ce.library_paths()
     cmd = ["g++", "-O1", "-std=c++17", "-shared", "-fPIC"] + srcs + objs + ["-o", out + ".tmp", "-I" + sysconfig.get_paths()["include"],
-           "-DTORCH_EXTENSION_NAME=_bde_host_emu", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           f"-DTORCH_EXTENSION_NAME={os.path.basename(out)[:-3]}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-Wl,-Bsymbolic"]
     cmd += ["-I" + i for i in ce.include_paths()] + ["-L" + l for l in libs]
     cmd += ["-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lpthread", "-Wl,-rpath," + libs[0]]
@@ -197,7 +197,7 @@ def load_host_nodes(sources):
     import importlib.util
     import torch  # noqa: F401
     path = build_host_nodes(sources)
-    spec = importlib.util.spec_from_file_location("_bde_host_emu", path)
+    spec = importlib.util.spec_from_file_location(os.path.basename(path)[:-3], path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     import ctypes
